@@ -52,6 +52,13 @@ typedef enum {
 #define TQ4_DEV_TIMEOUT 4   /* a bounded device-side wait gave up                */
 #define TQ4_DEV_WRITE_ORDER 8 /* tq4_write_and_attention: a new token's slot is not the last position of its
                                  sequence; it was written, but this call's attention may not have seen it */
+#define TQ4_DEV_PAGE_CONFLICT 16 /* tq4_copy_blocks: a page is the destination of two pairs with different sources, or
+                                    the source of one and the destination of another; the later pair, or the one that
+                                    reads it, was not carried out */
+#define TQ4_DEV_KEEP_ORDER 32 /* tq4_compact_rows: a list is not strictly increasing from 0 or more, or longer than its
+                                 row; its sequence was left as it is */
+#define TQ4_DEV_BAD_TREE 128 /* tq4_tree_mask: a parent that is no earlier draft of its sequence (taken for none), or a
+                               draft behind the mask's last bit */
 
 /* Library identification: returns e.g. "tq4-sm100a 0.1". Host call. */
 const char* tq4_version(void);
@@ -350,6 +357,90 @@ int tq4_paged_attention_static(const void* q, int q_dtype, int64_t num_rows, int
                                const float* rotation, float sm_scale, int causal, int sliding_window,
                                void* out, int out_dtype, int64_t out_token_stride,
                                int64_t out_head_stride, int mode, int* err_flag, void* stream);
+
+/*
+ * Rotary positions of queries and keys, in front of the cache write (no counterpart in the reference, whose callers hand over
+ * rotated vectors).  The pair (x, y) of frequency i at position p becomes f (x cos a - y sin a, y cos a + x sin a) with a = p *
+ * inv_freq[i], the exact product; pairs are dimensions (i, i + rotary_dim / 2), or (2 i, 2 i + 1) with `interleaved`; those from
+ * rotary_dim on are handed through.  inverse: -a, which undoes the rotation of f = 1 and is also its gradient.
+ * q, k [n_tokens, heads, head_dim] of one type (element strides {token, head}, innermost 1); either may have no heads.  An output
+ * may be its input (same pointer and strides) but not overlap it otherwise.  positions int32 / int64 [n_tokens], of any sign;
+ * inv_freq fp32 / fp64 [rotary_dim / 2], rotary_dim even, at most head_dim and 1024.  head_dim: any.
+ */
+int tq4_rotary(const void* q, const void* k, int dtype, int64_t n_tokens, int num_q_heads, int num_k_heads, int head_dim,
+               const int64_t* q_strides, const int64_t* k_strides, const void* positions, int positions_64,
+               const void* inv_freq, int inv_freq_64, int rotary_dim, int interleaved, float attention_factor, int inverse,
+               void* q_out, void* k_out, const int64_t* q_out_strides, const int64_t* k_out_strides, void* stream);
+
+/*
+ * Masks of trees of drafted tokens (no counterpart in the reference).  Sequence i's drafts are rows [query_start_loc[i],
+ * query_start_loc[i + 1]); parents[r] is the place, among its sequence's drafts, of the draft that row r continues, or -1 for one
+ * that continues the tokens held; it is earlier than the row's own.  mask int32 [num_rows, words]: bit k % 32 of word k / 32 is set
+ * where draft k is the row itself or an ancestor; depth int32 [num_rows]: how many ancestors (position minus tokens held).
+ * Rows past the last offset get zeros and -1.
+ */
+int tq4_tree_mask(const int32_t* parents, const int32_t* query_start_loc, int64_t num_rows, int num_seqs, int words,
+                  int32_t* mask, int32_t* depth, int* err_flag, void* stream);
+
+/*
+ * Attention of trees of drafted tokens over the packed cache (no counterpart in the reference).  Sequence i's drafts are query rows
+ * [query_start_loc[i], query_start_loc[i + 1]), T of them; their keys and values are in the cache already, at the last T of its
+ * seq_lens[i] positions.  A row sees every key in front of the drafts and draft k where bit k % 32 of word k / 32 of its mask is set
+ * (tq4_tree_mask makes such masks; any others are as good, also one without the row itself, or without any bit).  Drafts behind the
+ * mask's last bit are seen by no row.  sliding_window > 0: the row's position is the number of keys in front of the drafts plus that
+ * of its set bits, minus 1, and of the former it sees those within the window; the drafts are the mask's alone.
+ * tree_mask int32 [num_rows, tree_mask_words] and block_table int32 [num_seqs, bt_width] with row strides in elements; a sequence
+ * longer than its row of the table is cut there (TQ4_DEV_BAD_BLOCK).  max_seq_len as in tq4_attention_step; the other arguments,
+ * checks and the precision are those of tq4_paged_attention in the prefill form, with at most 128 query heads per KV head.  A row that
+ * sees no key, or past the last offset, gets zeros and an lse of -inf.
+ * workspace >= tq4_tree_attention_workspace_bytes(num_rows, Hq, Hkv, D), 16-byte aligned.
+ */
+size_t tq4_tree_attention_workspace_bytes(int64_t max_query_rows, int num_q_heads, int num_kv_heads, int head_dim);
+int tq4_tree_attention(const void* q, int q_dtype, int64_t num_rows, int num_seqs,
+                       int num_q_heads, int num_kv_heads, int head_dim,
+                       int64_t q_token_stride, int64_t q_head_stride,
+                       const uint8_t* cache, int64_t cache_block_stride, int64_t cache_token_stride,
+                       int64_t num_blocks, int block_size,
+                       const int32_t* block_table, int64_t bt_stride, int64_t bt_width,
+                       const int32_t* seq_lens, const int32_t* query_start_loc, int64_t max_seq_len,
+                       const int32_t* tree_mask, int64_t tree_mask_stride, int tree_mask_words,
+                       const float* k_centroids, int n_k_centroids,
+                       const float* v_centroids, int n_v_centroids,
+                       const float* rotation, float sm_scale, int sliding_window,
+                       void* out, int out_dtype, int64_t out_token_stride, int64_t out_head_stride,
+                       float* lse_out, int out_rotated,
+                       void* workspace, size_t workspace_bytes, int* err_flag, void* stream);
+
+/*
+ * Pages copied inside the caches of all layers (no counterpart in the reference): for every pair (source, destination) the token rows
+ * of page `source` (their num_kv_heads * (head_dim + 8) bytes of data) become those of page `destination`, in each of num_caches
+ * caches.  `caches`: HOST array of device pointers; the caches are alike (num_blocks pages, strides in bytes).  pairs int32 /
+ * int64 [n_pairs, 2] on the device.  A page may be the destination of one pair only and not also a source (other than of itself,
+ * which does nothing): of several pairs with one destination the first counts, and a pair whose source is another's destination
+ * is not carried out; both raise TQ4_DEV_PAGE_CONFLICT, unless the pairs are equal.  A page out of range raises TQ4_DEV_BAD_BLOCK.
+ * workspace: tq4_copy_blocks_workspace_bytes (0 for up to 1024 pairs: may be null).
+ */
+size_t tq4_copy_blocks_workspace_bytes(int64_t n_pairs, int64_t num_blocks);
+int tq4_copy_blocks(uint8_t* const* caches, int num_caches, int64_t num_blocks, int block_size, int64_t cache_block_stride,
+                    int64_t cache_token_stride, int num_kv_heads, int head_dim, const void* pairs, int pairs_64,
+                    int64_t n_pairs, void* workspace, size_t workspace_bytes, int* err_flag, void* stream);
+
+/*
+ * Token rows that stay, moved together inside the caches of all layers (no counterpart in the reference): for j < keep_lens[i] the row
+ * at position starts[i] + keep[i][j] of sequence i goes to position starts[i] + j, through the block table.  keep[i] is strictly
+ * increasing from 0 or more (the accepted path of a tree of drafts, or what an eviction leaves).  Rows behind the last one stay as they
+ * are.  The pages from position starts[i] on belong to sequence i alone.  seq_lens_out (optional) int32 [num_seqs] = starts + keep_lens;
+ * it may not overlap them.  block_table int32 [num_seqs, bt_width], keep int32 [num_seqs, keep_width] (row strides in elements).
+ * A list out of order, or keep_lens[i] outside 0 .. keep_width, leaves the sequence as it is (TQ4_DEV_KEEP_ORDER); rows in pages out
+ * of range, or past the table, are skipped (TQ4_DEV_BAD_BLOCK).
+ * workspace: tq4_compact_rows_workspace_bytes, 16-byte aligned (0 for up to 64 places a list: may be null).
+ */
+size_t tq4_compact_rows_workspace_bytes(int num_caches, int num_seqs, int keep_width, int num_kv_heads, int head_dim);
+int tq4_compact_rows(uint8_t* const* caches, int num_caches, int64_t num_blocks, int block_size, int64_t cache_block_stride,
+                     int64_t cache_token_stride, int num_kv_heads, int head_dim, const int32_t* block_table,
+                     int64_t bt_stride, int64_t bt_width, int num_seqs, const int32_t* starts, const int32_t* keep,
+                     int64_t keep_stride, int keep_width, const int32_t* keep_lens, int32_t* seq_lens_out, void* workspace,
+                     size_t workspace_bytes, int* err_flag, void* stream);
 
 /*
  * Per-kernel timing aid (no counterpart in the reference, which times with torch.cuda.Event

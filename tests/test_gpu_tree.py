@@ -1,0 +1,376 @@
+"""Masks of trees of drafted tokens, and attention with them over the packed cache, against 64-bit arithmetic from the definitions."""
+
+import math
+import random
+
+import numpy as np
+import pytest
+import torch
+
+from tests.helpers import Prims, build_paged_case
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops(cuda_lib):
+    from turboquant_vllm.kernels import ops as _ops
+
+    return _ops
+
+
+def offsets(counts):
+    return torch.tensor(np.concatenate([[0], np.cumsum(counts)]), dtype=torch.int32)
+
+
+def random_parents(nodes, rng, reach=5):
+    return [rng.randint(max(-1, j - reach), j - 1) for n in nodes for j in range(n)]
+
+
+def ancestor_matrix(nodes, parents):
+    """Per sequence the bool matrix [T, T]: row j sees itself and its ancestors."""
+    out, first = [], 0
+    for n in nodes:
+        m = np.zeros((n, n), dtype=bool)
+        for j in range(n):
+            p = parents[first + j]
+            if 0 <= p < j:
+                m[j] = m[p]
+            m[j, j] = True
+        out.append(m)
+        first += n
+    return out
+
+
+def pack(matrices, words):
+    """Masks as words: [rows, words] int32 (bits past the last word are dropped)."""
+    rows = []
+    for m in matrices:
+        bits = np.zeros((m.shape[0], 32 * words), dtype=np.uint64)
+        keep = min(m.shape[1], 32 * words)
+        bits[:, :keep] = m[:, :keep]
+        word = (bits.reshape(m.shape[0], words, 32) << np.arange(32, dtype=np.uint64)).sum(axis=2)
+        rows.append(word.astype(np.uint32).view(np.int32).reshape(m.shape[0], words))
+    return torch.from_numpy(np.concatenate(rows)) if rows else torch.zeros(0, words, dtype=torch.int32)
+
+
+def reference(q, case, nodes, matrices, pr, hkv, bs, scale, window=None):
+    """float64: out [rows, Hq, D], lse [rows, Hq], and the rms of the visible scores."""
+    rows, hq, d = q.shape
+    group = hq // hkv
+    out = torch.zeros(rows, hq, d, dtype=torch.float64)
+    lse = torch.full((rows, hq), -math.inf, dtype=torch.float64)
+    kc, vc, rot = pr.kc.double(), pr.vc.double(), pr.rot.double()
+    squares = count = 0.0
+    r0 = 0
+    for i, (n, m) in enumerate(zip(nodes, matrices)):
+        length = int(case["seq_lens"][i])
+        base = length - n
+        pos = torch.arange(length)
+        held = case["cache"][case["block_table"][i, pos // bs].long(), pos % bs]
+        vec, at = [], 0
+        for cents in (kc, vc):
+            idx = held[:, at : at + hkv * d // 2].reshape(length, hkv, d // 2).long()
+            at += hkv * d // 2
+            norm = held[:, at : at + 4 * hkv].contiguous().view(torch.float32).double()
+            at += 4 * hkv
+            vec.append((cents[torch.stack((idx >> 4, idx & 15), dim=-1).flatten(2)] @ rot) * norm[..., None])
+        for j in range(n):
+            sees = torch.zeros(length, dtype=torch.bool)
+            low = max(0, base + int(m[j].sum()) - window) if window else 0
+            sees[low : max(base, 0)] = True
+            for k in np.nonzero(m[j])[0]:
+                if 0 <= base + k < length:
+                    sees[base + k] = True
+            if not sees.any():
+                continue
+            for h in range(hq):
+                s = vec[0][sees, h // group] @ q[r0 + j, h].double() * scale
+                squares, count = squares + float(s.square().sum()), count + s.numel()
+                lse[r0 + j, h] = torch.logsumexp(s, 0)
+                out[r0 + j, h] = torch.softmax(s, 0) @ vec[1][sees, h // group]
+        r0 += n
+    return out, lse, math.sqrt(squares / max(count, 1))
+
+
+# ---- masks -------------------------------------------------------------------------------------
+@pytest.mark.parametrize("nodes,reach", [
+    ([1], 1), ([0, 3, 0, 1], 3), ([31, 32, 33, 64, 65], 4), ([5, 24, 7, 200], 40), ([2500, 3], 2), ([700], 1),  # (a chain of 700)
+])
+def test_mask_is_the_ancestors(ops, nodes, reach):
+    parents = random_parents(nodes, random.Random(sum(nodes)), reach)
+    want = ancestor_matrix(nodes, parents)
+    widest = max(nodes)
+    mask, depth = ops.tq4_tree_mask(torch.tensor(parents, dtype=torch.int32).cuda(), offsets(nodes).cuda(), widest)
+    assert mask.dtype == depth.dtype == torch.int32 and mask.shape == (sum(nodes), -(-widest // 32))
+    assert torch.equal(mask.cpu(), pack(want, -(-widest // 32)))
+    assert depth.tolist() == [int(r.sum()) - 1 for m in want for r in m]
+    assert ops.read_and_clear_errors(mask.device) == 0
+
+
+def test_mask_of_rows_behind_the_last_sequence_and_of_bad_parents(ops):
+    from turboquant_vllm import _native as nv
+
+    starts = torch.tensor([0, 3], dtype=torch.int32).cuda()
+    mask, depth = ops.tq4_tree_mask(torch.tensor([-1, 0, 1, 0, -1], dtype=torch.int32).cuda(), starts, 40)
+    assert mask.tolist() == [[1, 0], [3, 0], [7, 0], [0, 0], [0, 0]] and depth.tolist() == [0, 1, 2, -1, -1]
+    assert ops.read_and_clear_errors(mask.device) == 0
+    # a parent that is the row itself, a later one, or below -1: the row starts a branch, and it is reported
+    for bad in (1, 2, -2, 1 << 30):
+        mask, depth = ops.tq4_tree_mask(torch.tensor([-1, bad, 1], dtype=torch.int32).cuda(), starts, 3)
+        assert mask.flatten().tolist() == [1, 2, 6] and depth.tolist() == [0, 0, 1]
+        assert ops.read_and_clear_errors(mask.device) == nv.DEV_BAD_TREE
+    # a draft without a bit of its own
+    parents = torch.tensor([-1] + list(range(39)), dtype=torch.int32).cuda()
+    mask, depth = ops.tq4_tree_mask(parents, torch.tensor([0, 40], dtype=torch.int32).cuda(), 32)
+    assert mask.shape == (40, 1) and mask[39].item() == -1 and depth[39].item() == 39
+    assert ops.read_and_clear_errors(mask.device) == nv.DEV_BAD_TREE
+
+
+def test_mask_refusals(ops):
+    starts, parents = torch.tensor([0, 2], dtype=torch.int32).cuda(), torch.tensor([-1, 0], dtype=torch.int32).cuda()
+    with pytest.raises(AssertionError, match="parents"):
+        ops.tq4_tree_mask(parents.long(), starts, 2)
+    with pytest.raises(AssertionError, match="query_start_loc"):
+        ops.tq4_tree_mask(parents, starts.long(), 2)
+    with pytest.raises(AssertionError, match="max_nodes"):
+        ops.tq4_tree_mask(parents, starts, 0)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.tq4_tree_mask(parents.cpu(), starts, 2)
+    mask, depth = ops.tq4_tree_mask(parents[:0], starts[:1], 7)
+    assert mask.shape == (0, 1) and depth.shape == (0,)
+
+
+# ---- attention ---------------------------------------------------------------------------------
+CASES = [  # head_dim, q heads, KV heads, lengths, drafts, block size, window, row format, query type
+    (128, 28, 4, [40], [8], 16, None, True, "bf16"),
+    (128, 4, 4, [1], [1], 16, None, True, "fp16"),                       # nothing held, one draft
+    (128, 8, 2, [7, 0, 300], [7, 0, 1], 16, None, True, "bf16"),         # drafts alone, an empty sequence, a single draft
+    (128, 32, 8, [700, 130, 64, 65], [16, 9, 24, 1], 16, None, True, "fp16"),
+    (128, 32, 8, [3000], [33], 16, None, True, "bf16"),                  # cut along the keys, two words
+    (128, 8, 2, [600, 90], [200, 70], 16, None, True, "bf16"),           # several row blocks beside one stream of two
+    (128, 28, 4, [500, 129], [37, 100], 32, None, False, "bf16"),        # groups of 7, rows without padding
+    (128, 4, 1, [333], [40], 256, None, False, "bf16"),                  # 136-byte rows
+    (64, 14, 2, [200, 1000], [30, 64], 16, None, True, "bf16"),
+    (64, 64, 1, [150], [9], 24, None, True, "fp16"),                     # a group of 64: two rows a block; pages that end in tiles
+    (96, 4, 4, [300, 41], [64, 9], 16, None, True, "bf16"),
+    (96, 32, 32, [257], [100], 16, None, "dense", "bf16"),
+    (256, 8, 4, [300, 90, 3], [12, 90, 3], 16, 64, True, "bf16"),
+    (256, 2, 2, [900], [17], 16, None, True, "fp16"),
+    (128, 8, 4, [500, 100, 20], [20, 33, 20], 16, 48, True, "bf16"),     # a window
+    (128, 8, 4, [500, 100], [20, 70], 16, 3, True, "bf16"),              # ... shorter than the branches
+    (128, 8, 8, [90], [40], 16, None, True, "fp32"),
+]
+DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
+
+
+def _call(ops, q, case, nodes, mask, p, hkv, bs, **kw):
+    return ops.paged_tq4_tree_attention(
+        q.cuda(), case["cache"].cuda(), case["block_table"].cuda(), case["seq_lens"].cuda(), offsets(nodes).cuda(), mask.cuda(), p["kc"],
+        p["vc"], p["rot"], hkv, bs, **kw)
+
+
+def _check(got, lse, want, want_lse, spread, out_dtype=torch.float32):
+    # Keys and values are centroids on the tensor cores' fp16 grid (half a step: 2^-11 of the value); an error of 2^-11 in a key moves
+    # its score, and with it its weight, by 2^-11 of the score.  16-bit outputs add half a step of their own.
+    tol = 2 ** -11 * (1 + spread) + (0 if out_dtype == torch.float32 else torch.finfo(out_dtype).eps / 2)
+    assert torch.isfinite(got).all()
+    assert (got.double() - want).norm() <= tol * want.norm() + 1e-30
+    if lse is not None:
+        seen = want_lse > -math.inf
+        assert torch.equal(lse > -math.inf, seen)
+        # (a score of `spread` moves by 2^-11 of it, at most some four times that for the largest; fp32 sums and log2 add 1e-5)
+        assert (lse.double() - want_lse)[seen].abs().max() <= 2 ** -11 * 4 * (1 + spread) + 1e-5 if seen.any() else True
+
+
+@pytest.mark.parametrize("d,hq,hkv,lens,nodes,bs,window,padded,dtype", CASES)
+def test_tree_attention(ops, d, hq, hkv, lens, nodes, bs, window, padded, dtype):
+    pr = Prims(d)
+    case = build_paged_case(lens, hkv, d, bs, pr, seed=5, padded=padded)
+    rng = random.Random(d + sum(lens))
+    matrices = ancestor_matrix(nodes, random_parents(nodes, rng))
+    q = torch.randn(sum(nodes), hq, d, generator=torch.Generator().manual_seed(1)).to(DTYPES[dtype])
+    lse = torch.full((sum(nodes), hq), math.nan, device="cuda")
+    got = _call(ops, q, case, nodes, pack(matrices, -(-max(nodes) // 32)), pr.cuda(), hkv, bs, sliding_window=window,
+                out_dtype=torch.float32, lse_out=lse)
+    want, want_lse, spread = reference(q, case, nodes, matrices, pr, hkv, bs, d ** -0.5, window)
+    _check(got.cpu(), lse.cpu(), want, want_lse, spread)
+    assert ops.read_and_clear_errors(got.device) == 0
+
+
+@pytest.mark.parametrize("d,hq,hkv,lens,nodes", [(128, 8, 2, [40, 30, 12], [20, 30, 12]), (256, 8, 4, [70, 5], [40, 5]), (64, 4, 4, [33], [33])])
+def test_any_mask_also_one_that_leaves_a_row_empty(ops, d, hq, hkv, lens, nodes):
+    """Masks that no tree has: rows without any bit, without their own, with later drafts."""
+    pr = Prims(d)
+    case = build_paged_case(lens, hkv, d, 16, pr, seed=8, padded=True)
+    rng = np.random.default_rng(d)
+    matrices = [rng.random((n, n)) < 0.3 for n in nodes]
+    for m in matrices:
+        m[::5] = False
+    q = torch.randn(sum(nodes), hq, d, generator=torch.Generator().manual_seed(2)).bfloat16()
+    lse = torch.empty(sum(nodes), hq, device="cuda")
+    got = _call(ops, q, case, nodes, pack(matrices, 2), pr.cuda(), hkv, 16, out_dtype=torch.float32, lse_out=lse)
+    want, want_lse, spread = reference(q, case, nodes, matrices, pr, hkv, 16, d ** -0.5)
+    _check(got.cpu(), lse.cpu(), want, want_lse, spread)
+    empty = (want_lse == -math.inf).all(dim=1)
+    assert empty.any() and (got.cpu()[empty] == 0).all()
+
+
+def test_drafts_behind_the_masks_last_bit_are_hidden(ops):
+    pr, nodes = Prims(128), [50]
+    case = build_paged_case([90], 2, 128, 16, pr, seed=3, padded=True)
+    matrices = ancestor_matrix(nodes, random_parents(nodes, random.Random(1), 3))
+    q = torch.randn(50, 8, 128, generator=torch.Generator().manual_seed(3)).half()
+    got = _call(ops, q, case, nodes, pack(matrices, 1), pr.cuda(), 2, 16, out_dtype=torch.float32)
+    matrices[0][:, 32:] = False
+    want, want_lse, spread = reference(q, case, nodes, matrices, pr, 2, 16, 128 ** -0.5)
+    _check(got.cpu(), None, want, want_lse, spread)
+    got = _call(ops, q, case, nodes, torch.zeros(50, 0, dtype=torch.int32), pr.cuda(), 2, 16, out_dtype=torch.float32)  # no bits at all
+    matrices[0][:] = False
+    want, want_lse, spread = reference(q, case, nodes, matrices, pr, 2, 16, 128 ** -0.5)
+    _check(got.cpu(), None, want, want_lse, spread)
+
+
+def test_more_drafts_than_tokens(ops):
+    """A length below the number of drafts: the first drafts have no keys."""
+    pr, nodes = Prims(128), [20]
+    case = build_paged_case([12], 2, 128, 16, pr, seed=3, padded=True)
+    matrices = ancestor_matrix(nodes, random_parents(nodes, random.Random(1), 3))
+    q = torch.randn(20, 4, 128, generator=torch.Generator().manual_seed(3)).half()
+    lse = torch.empty(20, 4, device="cuda")
+    got = _call(ops, q, case, nodes, pack(matrices, 1), pr.cuda(), 2, 16, out_dtype=torch.float32, lse_out=lse)
+    want, want_lse, spread = reference(q, case, nodes, matrices, pr, 2, 16, 128 ** -0.5)
+    _check(got.cpu(), lse.cpu(), want, want_lse, spread)
+
+
+@pytest.mark.parametrize("d,hq,hkv,length,n", [(128, 32, 8, 900, 12), (256, 8, 4, 333, 20), (64, 14, 2, 2000, 40)])
+def test_a_chain_is_causal_attention(ops, d, hq, hkv, length, n):
+    """A tree that is one branch: the chunked prefill of the same rows."""
+    pr = Prims(d)
+    p = pr.cuda()
+    case = build_paged_case([length], hkv, d, 16, pr, seed=9, padded=True)
+    q = torch.randn(n, hq, d, generator=torch.Generator().manual_seed(4)).bfloat16()
+    mask, _ = ops.tq4_tree_mask(torch.arange(-1, n - 1, dtype=torch.int32).cuda(), offsets([n]).cuda(), n)
+    got = _call(ops, q, case, [n], mask, p, hkv, 16, out_dtype=torch.float32)
+    want = ops.paged_tq4_attention(q.cuda(), case["cache"].cuda(), case["block_table"].cuda(), case["seq_lens"].cuda(), p["kc"], p["vc"],
+                                   p["rot"], hkv, 16, query_start_loc=offsets([n]).cuda(), out_dtype=torch.float32)
+    # (the same tables and two-term products; sums in tensor memory truncate, at most 8 * 2^-23 a tile of 64 keys, as in the prefill kernel)
+    assert (got - want).norm() <= (8 * (length / 64 + 1) * 2 ** -23 + 2 ** -18) * want.norm()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_16bit_output_strided_queries_and_rows_behind_the_last_sequence(ops, dtype):
+    pr, nodes = Prims(128), [9, 5]
+    p = pr.cuda()
+    case = build_paged_case([200, 77], 2, 128, 16, pr, seed=3, padded=True)
+    matrices = ancestor_matrix(nodes, random_parents(nodes, random.Random(1), 3))
+    fused = torch.randn(17, 8 + 4, 128, generator=torch.Generator().manual_seed(3)).to(DTYPES[dtype])  # q | k | v of a projection
+    mask = torch.cat((pack(matrices, 1), torch.full((3, 1), -1, dtype=torch.int32)))
+    out = torch.full((17, 8, 160), 7.0, dtype=DTYPES[dtype], device="cuda")
+    q = fused.cuda()[:, :8]
+    got = ops.paged_tq4_tree_attention(q, case["cache"].cuda(), case["block_table"].cuda(), case["seq_lens"].cuda(), offsets(nodes).cuda(),
+                                       mask.cuda(), p["kc"], p["vc"], p["rot"], 2, 16, out=out[..., :128])
+    assert got.data_ptr() == out.data_ptr() and (out[..., 128:] == 7).all()
+    full = _call(ops, fused[:, :8].contiguous(), case, nodes, mask, p, 2, 16, out_dtype=torch.float32)
+    assert torch.equal(out[..., :128], full.to(out.dtype))
+    want, want_lse, spread = reference(fused[:14, :8], case, nodes, matrices, pr, 2, 16, 128 ** -0.5)
+    _check(out[:14, :, :128].cpu(), None, want, want_lse, spread, DTYPES[dtype])
+    assert (out[14:, :, :128] == 0).all()
+
+
+def test_rotated_output_and_its_merge(ops):
+    """Rotated partials with their lse, as the shards of a long context are merged."""
+    pr, nodes = Prims(128), [12]
+    p = pr.cuda()
+    case = build_paged_case([700], 4, 128, 16, pr, seed=3, padded=True)
+    matrices = ancestor_matrix(nodes, random_parents(nodes, random.Random(1), 3))
+    q = torch.randn(12, 8, 128, generator=torch.Generator().manual_seed(3)).half()
+    lse = torch.empty(12, 8, device="cuda")
+    rotated = _call(ops, q, case, nodes, pack(matrices, 1), p, 4, 16, out_dtype=torch.float32, lse_out=lse, out_rotated=True)
+    got = ops.combine_partials(rotated[None], lse[None], p["rot"])
+    want, _, spread = reference(q, case, nodes, matrices, pr, 4, 16, 128 ** -0.5)
+    _check(got.cpu(), None, want, None, spread)
+
+
+def test_bad_pages_and_lengths_are_reported_and_hidden(ops):
+    from turboquant_vllm import _native as nv
+
+    pr, nodes = Prims(128), [6]
+    p = pr.cuda()
+    case = build_paged_case([100], 2, 128, 16, pr, seed=3, padded=True)
+    matrices = ancestor_matrix(nodes, random_parents(nodes, random.Random(1), 3))
+    q = torch.randn(6, 8, 128, generator=torch.Generator().manual_seed(3)).half()
+    mask = pack(matrices, 1)
+    good = _call(ops, q, case, nodes, mask, p, 2, 16, out_dtype=torch.float32)
+    bad = dict(case, block_table=case["block_table"].clone())
+    bad["block_table"][0, 2] = 1 << 30
+    out = _call(ops, q, bad, nodes, mask, p, 2, 16, out_dtype=torch.float32)
+    assert ops.read_and_clear_errors(out.device) == nv.DEV_BAD_BLOCK
+    assert torch.isfinite(out).all() and not torch.equal(out, good)
+    # a length past the table's row is cut there; the row stride may be wider than the row
+    wide = torch.zeros(1, 64, dtype=torch.int32)
+    wide[0, :7] = case["block_table"][0, :7]
+    far = dict(case, seq_lens=torch.tensor([500], dtype=torch.int32))
+    out = ops.paged_tq4_tree_attention(q.cuda(), case["cache"].cuda(), wide.cuda()[:, :7], far["seq_lens"].cuda(), offsets(nodes).cuda(),
+                                       mask.cuda(), p["kc"], p["vc"], p["rot"], 2, 16, out_dtype=torch.float32)
+    assert ops.read_and_clear_errors(out.device) == nv.DEV_BAD_BLOCK and torch.isfinite(out).all()
+
+
+def test_refusals(ops):
+    pr, nodes = Prims(128), [6]
+    p = pr.cuda()
+    case = build_paged_case([100], 2, 128, 16, pr, seed=3, padded=True)
+    q, mask = torch.zeros(6, 8, 128, dtype=torch.float16), torch.zeros(6, 1, dtype=torch.int32)
+
+    def call(error, match, q=q, case=case, mask=mask, hkv=2, bs=16, starts=offsets(nodes), **kw):
+        with pytest.raises(error, match=match):
+            ops.paged_tq4_tree_attention(q.cuda(), case["cache"].cuda(), case["block_table"].cuda(), case["seq_lens"].cuda(),
+                                         starts.cuda(), mask.cuda(), p["kc"], p["vc"], p["rot"], hkv, bs, **kw)
+
+    call(AssertionError, "tree_mask", mask=mask[:5])
+    call(AssertionError, "tree_mask", mask=mask.long())
+    call(AssertionError, "multiple of the KV heads", hkv=3)
+    call(AssertionError, "block_size", bs=32)
+    call(AssertionError, "query_start_loc", starts=offsets([3, 3]))
+    call(AssertionError, "seq_lens", case=dict(case, seq_lens=case["seq_lens"].long()))
+    call(AssertionError, "out must", out=torch.empty(6, 8, 64, device="cuda"))
+    call(ValueError, "workspace has", workspace=torch.empty(64, dtype=torch.uint8, device="cuda"))
+    call(AssertionError, "rotation", q=torch.zeros(6, 8, 80, dtype=torch.float16))
+    call(TypeError, "float32/float16/bfloat16", q=q.double())
+    with pytest.raises(ValueError):
+        ops.tree_attention_workspace_bytes(4, 129, 1, 128)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.paged_tq4_tree_attention(q, case["cache"].cuda(), case["block_table"].cuda(), case["seq_lens"].cuda(), offsets(nodes).cuda(),
+                                     mask.cuda(), p["kc"], p["vc"], p["rot"], 2, 16)
+
+
+def test_captured_calls_on_two_streams_and_an_own_workspace(ops):
+    """Two captured graphs, replayed on two streams at a time, give what eager calls give; so does a workspace of the caller's."""
+    pr = Prims(128)
+    p = pr.cuda()
+    cases = []
+    for seed, lens, nodes in ((1, [900, 40], [7, 20]), (2, [64, 2000], [64, 3])):
+        case = build_paged_case(lens, 2, 128, 16, pr, seed=seed, padded=True)
+        matrices = ancestor_matrix(nodes, random_parents(nodes, random.Random(seed), 3))
+        q = torch.randn(sum(nodes), 8, 128, generator=torch.Generator().manual_seed(seed)).half().cuda()
+        args = [q, case["cache"].cuda(), case["block_table"].cuda(), case["seq_lens"].cuda(), offsets(nodes).cuda(), pack(matrices, 2).cuda(),
+                p["kc"], p["vc"], p["rot"], 2, 16]
+        out = torch.empty(sum(nodes), 8, 128, device="cuda")
+        eager = ops.paged_tq4_tree_attention(*args, out_dtype=torch.float32)
+        ws = torch.empty(ops.tree_attention_workspace_bytes(sum(nodes), 8, 2, 128), dtype=torch.uint8, device="cuda")
+        assert torch.equal(ops.paged_tq4_tree_attention(*args, out_dtype=torch.float32, workspace=ws), eager)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            ops.paged_tq4_tree_attention(*args, out=out)
+        cases.append((graph, out, eager, torch.cuda.Stream(), args))  # (the graph reads its inputs where they are)
+    for _ in range(3):
+        for _, out, *_ in cases:
+            out.fill_(math.nan)
+        torch.cuda.synchronize()
+        for graph, _, _, stream, _ in cases:
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for _, out, eager, *_ in cases:
+            assert torch.equal(out, eager)

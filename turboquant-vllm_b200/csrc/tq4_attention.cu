@@ -892,28 +892,6 @@ int launch_attention_fp32(const AttnArgs& a, cudaStream_t st) {
 // 3. Merge the partials of a row, normalise, un-rotate, store.
 //    Also serves tq4_combine_partials (cross-GPU shards) through the "dense" mode.
 // ======================================================================================
-struct CombineArgs {
-  const int* active_rows;  // (optional) device count: only the first so many rows are merged ...
-  const int* row_end;      // (optional) last visible key of the rows: -1 = a row of the prefill kernel
-  int rows_long;           // with row_end: merge the prefill kernel's rows (1) or the others (0)
-  // sparse mode (slot_base != null): the partials of row r are slot_base[r]..slot_base[r+1], x TPC
-  const int* slot_base;
-  int TPC;
-  const float* part_o;
-  const float* part_m;
-  const float* part_l;
-  // dense mode (slot_base == null): `world` parts, part index w*rows + r; part_m holds natural-log
-  // LSE and part_o is already normalised
-  int world;
-  int rows, row_offset, Hq;
-  const float* rotation;
-  void* out;
-  int out_dtype;
-  int64_t out_token_stride, out_head_stride;
-  float* lse_out;
-  int out_rotated;
-};
-
 // Merge kernel: eight warps, VB = 8 / WPV (row, head) vectors per pass.
 //   1. WPV warps merge the partials of one vector: warp w takes partials w, w + WPV, ..., a lane holds
 //      the maximum and sum of one of them and four (D = 256: eight) of the accumulator's coordinates, so

@@ -100,14 +100,20 @@ struct AttnArgs {
   int no_plan;       // the prologue rotates (and writes) only, its queries are fp16 terms (tq4_decode_step.cu)
   int plan_records;  // the plan writes row_rec and span_rec (tensor-core kernel)
   int fused;  // tensor-core kernel: compute the tile plan and rotate the queries inside the kernel
+  // tree calls (tq4_tree_attention): which drafts a row sees, bit k % 32 of word k / 32 of its mask (else null)
+  const int32_t* tree_mask;
+  int64_t tree_stride;
+  int tree_words;
+  int64_t table_width;  // blocks of a row of the table
   const CompressArgs* fused_write;  // host side only: the step's cache write, done inside the fused kernel
 };
 
 // A sequence cannot be longer than its block-table row (the C interface carries the row stride, not
-// the row's width: the stride bounds it).  A longer seq_len is cut there and reported, so no kernel
+// the row's width, except in tree calls: the stride bounds it).  A longer seq_len is cut there and reported, so no kernel
 // reads a page id past the row.
+template <bool WIDTH = false>
 __device__ __forceinline__ int clamp_seq_len(const AttnArgs& a, int len) {
-  const long long cap = (long long)a.bt_stride * a.block_size;
+  const long long cap = (long long)(WIDTH ? a.table_width : a.bt_stride) * a.block_size;
   if ((long long)len > cap) {
     if (a.err_flag) atomicOr(a.err_flag, TQ4_DEV_BAD_BLOCK);
     len = (int)cap;
@@ -161,6 +167,30 @@ inline size_t carve_plan(AttnPlan& p, void* ws, int64_t rows, int Hq, int D, int
   return off;
 }
 
+// Merge of the partials of a row (tq4_attention.cu).
+struct CombineArgs {
+  const int* active_rows;  // (optional) device count: only the first so many rows are merged ...
+  const int* row_end;      // (optional) last visible key of the rows: -1 = a row of the prefill kernel
+  int rows_long;           // with row_end: merge the prefill kernel's rows (1) or the others (0)
+  // sparse mode (slot_base != null): the partials of row r are slot_base[r]..slot_base[r+1], x TPC
+  const int* slot_base;
+  int TPC;
+  const float* part_o;
+  const float* part_m;
+  const float* part_l;
+  // dense mode (slot_base == null): `world` parts, part index w*rows + r; part_m holds natural-log
+  // LSE and part_o is already normalised
+  int world;
+  int rows, row_offset, Hq;
+  const float* rotation;
+  void* out;
+  int out_dtype;
+  int64_t out_token_stride, out_head_stride;
+  float* lse_out;
+  int out_rotated;
+};
+int launch_combine(const CombineArgs& c, int D, cudaStream_t st, bool pdl);
+
 // Launchers implemented in tq4_attention.cu / tq4_decode_mma.cu.
 int launch_attention_fp32(const AttnArgs& a, cudaStream_t st);
 int launch_attention_mma(const AttnArgs& a, cudaStream_t st);  // returns TQ4_ERR_UNSUPPORTED if shape not covered
@@ -181,6 +211,9 @@ int prefill_tc_splits(const AttnArgs& a, int64_t slots);
 size_t prefill_tc_image_bytes(int D);
 int launch_prefill_tc(const AttnArgs& a, cudaStream_t st, bool fast, int min_rows, int splits, bool to_parts,
                       uint8_t* image, float* part_o, float* part_m);
+// the same kernel with the masks of a tree call (a.tree_mask); every sequence's rows, in `splits` key parts
+int tree_tc_splits(const AttnArgs& a, int64_t slots);
+int launch_tree_tc(const AttnArgs& a, cudaStream_t st, int splits, bool to_parts, uint8_t* image, float* part_o, float* part_m);
 constexpr int kPrefillMinRows = 8;  // new rows of a sequence from which the prefill kernel is the faster one
 int mma_warps_per_cta(int D, int GC, int Hkv, int64_t token_stride = 0);
 bool attention_mma_supported(const AttnShape& sh, int block_size, const uint8_t* cache,

@@ -104,6 +104,13 @@ void check(int status, const char* what) {
   fail(PyExc_RuntimeError, msg + " (tq4 status " + std::to_string(status) + ")");
 }
 
+// A tensor of a call whose kernels run on device `dev`: one elsewhere is not read through its address
+const at::Tensor& on_device(const at::Tensor& t, int dev, const char* name) {
+  if (t.get_device() != dev)
+    fail(PyExc_RuntimeError, std::string(name) + " is on " + t.device().str() + ", the call runs on cuda:" + std::to_string(dev));
+  return t;
+}
+
 // Attention scratch of the callers that bring none, grown on demand.  A call is several launches that hand data
 // on through it, made without the GIL, so no two calls that can run at a time may share one: it belongs to a
 // stream (kernels of two streams overlap) and a thread (launches of two threads interleave).  The last
@@ -602,6 +609,330 @@ PyObject* cache_step(PyObject*, PyObject* const* p, Py_ssize_t n) {
   });
 }
 
+// tree_attention(q, kv_cache, block_table, seq_lens, query_start_loc, tree_mask, k_centroids, v_centroids, rotation, num_kv_heads, block_size,
+//                sm_scale, sliding_window, out, out_dtype, lse_out, out_rotated, workspace, max_seq_len)
+PyObject* tree_attention(PyObject*, PyObject* const* p, Py_ssize_t n) {
+  if (!expect("tree_attention", n, 19)) return nullptr;
+  return guarded([&]() -> PyObject* {
+    at::Tensor q = cuda_tensor(p[0], "q");
+    const int dev = device_index(q);
+    auto input = [&](int i, const char* name) -> const at::Tensor& { return on_device(cuda_tensor(p[i], name), dev, name); };
+    const at::Tensor &cache = input(1, "kv_cache"), &bt = input(2, "block_table"), &lens = input(3, "seq_lens");
+    const at::Tensor &qsl = input(4, "query_start_loc"), &mask = input(5, "tree_mask");
+    const at::Tensor &kc = input(6, "k_centroids"), &vc = input(7, "v_centroids");
+    at::Tensor rot = input(8, "rotation");
+    const int64_t hkv = as_int(p[9]), block = as_int(p[10]);
+    TQ4_ASSERT(q.dim() == 3, "q must have three dimensions");
+    const int64_t t = q.size(0), hq = q.size(1), d = q.size(2);
+    TQ4_ASSERT(hkv > 0 && hq % hkv == 0, "query heads must be a multiple of the KV heads");
+    TQ4_ASSERT(cache.scalar_type() == at::kByte && cache.dim() == 3 && cache.stride(2) == 1 && block > 0 && cache.size(1) == block,
+               "kv_cache must be uint8 [blocks, block_size, bytes] with contiguous rows");
+    TQ4_ASSERT(lens.scalar_type() == at::kInt && lens.dim() == 1 && lens.is_contiguous(), "seq_lens must be contiguous int32");
+    TQ4_ASSERT(bt.scalar_type() == at::kInt && bt.dim() == 2 && bt.size(0) >= lens.numel() && (bt.size(1) < 2 || bt.stride(1) == 1),
+               "block_table must be int32 [sequences, blocks] with contiguous rows");
+    TQ4_ASSERT(qsl.scalar_type() == at::kInt && qsl.is_contiguous() && qsl.numel() == lens.numel() + 1,
+               "query_start_loc must be contiguous int32 [sequences + 1]");
+    TQ4_ASSERT(mask.scalar_type() == at::kInt && mask.dim() == 2 && mask.size(0) == t && (mask.size(1) < 2 || mask.stride(1) == 1),
+               "tree_mask must be int32 [rows, words] with contiguous rows");
+    TQ4_ASSERT(rot.scalar_type() == at::kFloat && rot.numel() == d * d, "rotation must be float32 [head_dim, head_dim]");
+    TQ4_ASSERT(kc.scalar_type() == at::kFloat && vc.scalar_type() == at::kFloat && kc.is_contiguous() && vc.is_contiguous(),
+               "centroids must be contiguous float32");
+    if (!rot.is_contiguous()) rot = rot.contiguous();
+    q = inner_contiguous(q);
+    const float scale = p[11] == Py_None ? (float)(1.0 / std::sqrt((double)d)) : (float)as_double(p[11]);
+    const int window = (int)int_or_zero(p[12]);
+    Launch launch(dev);
+    at::Tensor out;
+    const bool own_out = p[13] == Py_None;
+    if (own_out) {
+      const at::ScalarType dt = p[14] == Py_None ? q.scalar_type() : as_dtype(p[14]);
+      out = at::empty({t, hq, d}, q.options().dtype(dt).requires_grad(false));
+    } else {
+      out = input(13, "out");
+      TQ4_ASSERT(out.dim() == 3 && out.size(0) == t && out.size(1) == hq && out.size(2) == d && out.stride(2) == 1,
+                 "out must have q's shape and contiguous rows");
+    }
+    float* lse = nullptr;
+    if (p[15] != Py_None) {
+      const at::Tensor& l = input(15, "lse_out");
+      TQ4_ASSERT(l.scalar_type() == at::kFloat && l.is_contiguous() && l.numel() >= t * hq,
+                 "lse_out must be contiguous float32 of rows x heads");
+      lse = (float*)l.data_ptr();
+    }
+    const size_t need = tq4_tree_attention_workspace_bytes(t > 1 ? t : 1, (int)hq, (int)hkv, (int)d);
+    if (need == 0)
+      fail(PyExc_ValueError, "unsupported attention shape: Hq=" + std::to_string(hq) + ", Hkv=" + std::to_string(hkv) +
+                                 ", D=" + std::to_string(d));
+    const at::Tensor ws = p[17] == Py_None ? workspace_of(dev, launch.stream, (int64_t)need) : input(17, "workspace");
+    const size_t have = (size_t)ws.numel() * ws.element_size();
+    if (have < need)
+      fail(PyExc_ValueError, "workspace has " + std::to_string(have) + " bytes, " + std::to_string(need) + " needed");
+    int64_t max_seq_len = p[18] == Py_None ? 0 : as_int(p[18]);
+    if (bt.size(1) > 0 && (max_seq_len <= 0 || max_seq_len > bt.size(1) * block)) max_seq_len = bt.size(1) * block;
+    const int rotated = truth(p[16]) ? 1 : 0;
+    int* flag = (int*)flag_of(dev).data_ptr();
+    const int q_dt = dtype_code(q.scalar_type()), out_dt = dtype_code(out.scalar_type());
+    int st;
+    {
+      const NoGil no_gil;
+      st = tq4_tree_attention(
+          q.data_ptr(), q_dt, t, (int)lens.numel(), (int)hq, (int)hkv, (int)d, q.stride(0), q.stride(1),
+          (const uint8_t*)cache.data_ptr(), cache.stride(0), cache.stride(1), cache.size(0), (int)block, (const int32_t*)bt.data_ptr(),
+          bt.stride(0), bt.size(1), (const int32_t*)lens.data_ptr(), (const int32_t*)qsl.data_ptr(), max_seq_len, (const int32_t*)mask.data_ptr(),
+          mask.stride(0), (int)mask.size(1), (const float*)kc.data_ptr(), (int)kc.numel(), (const float*)vc.data_ptr(), (int)vc.numel(),
+          (const float*)rot.data_ptr(), scale, window, out.data_ptr(), out_dt, out.stride(0), out.stride(1), lse, rotated, ws.data_ptr(),
+          have, flag, launch.stream);
+    }
+    check(st, "paged_tq4_tree_attention");
+    if (!own_out) {
+      Py_INCREF(p[13]);
+      return p[13];
+    }
+    return THPVariable_Wrap(std::move(out));
+  });
+}
+
+// tree_mask(parents, query_start_loc, max_nodes) -> (mask, depth)
+PyObject* tree_mask(PyObject*, PyObject* const* p, Py_ssize_t n) {
+  if (!expect("tree_mask", n, 3)) return nullptr;
+  return guarded([&]() -> PyObject* {
+    const at::Tensor& parents = cuda_tensor(p[0], "parents");
+    const int dev = device_index(parents);
+    const at::Tensor& qsl = on_device(cuda_tensor(p[1], "query_start_loc"), dev, "query_start_loc");
+    const int64_t nodes = as_int(p[2]);
+    TQ4_ASSERT(parents.scalar_type() == at::kInt && parents.dim() == 1 && parents.is_contiguous(), "parents must be contiguous int32 [rows]");
+    TQ4_ASSERT(qsl.scalar_type() == at::kInt && qsl.dim() == 1 && qsl.is_contiguous() && qsl.numel() > 0,
+               "query_start_loc must be contiguous int32 [sequences + 1]");
+    TQ4_ASSERT(nodes > 0 && nodes <= (1 << 20), "max_nodes must be between 1 and 2^20");
+    const int64_t rows = parents.numel(), words = (nodes + 31) / 32;
+    Launch launch(dev);
+    at::Tensor mask = at::empty({rows, words}, parents.options().requires_grad(false));
+    at::Tensor depth = at::empty({rows}, parents.options().requires_grad(false));
+    int* flag = (int*)flag_of(dev).data_ptr();
+    int st;
+    {
+      const NoGil no_gil;
+      st = tq4_tree_mask((const int32_t*)parents.data_ptr(), (const int32_t*)qsl.data_ptr(), rows, (int)qsl.numel() - 1, (int)words,
+                         (int32_t*)mask.data_ptr(), (int32_t*)depth.data_ptr(), flag, launch.stream);
+    }
+    check(st, "tq4_tree_mask");
+    PyObject* pair = PyTuple_New(2);
+    if (!pair) throw PyError{};
+    PyTuple_SET_ITEM(pair, 0, THPVariable_Wrap(std::move(mask)));
+    PyTuple_SET_ITEM(pair, 1, THPVariable_Wrap(std::move(depth)));
+    return pair;
+  });
+}
+
+// bytes [first, last) that a tensor's elements lie in
+void byte_range(const at::Tensor& t, uintptr_t& first, uintptr_t& last) {
+  int64_t lo = 0, hi = 0;
+  for (int64_t i = 0; i < t.dim(); ++i) (t.stride(i) < 0 ? lo : hi) += (t.size(i) - 1) * t.stride(i);
+  first = (uintptr_t)t.data_ptr() + lo * (int64_t)t.element_size();
+  last = (uintptr_t)t.data_ptr() + (hi + 1) * (int64_t)t.element_size();
+}
+bool overlap(const at::Tensor& a, const at::Tensor& b) {
+  if (a.numel() == 0 || b.numel() == 0) return false;
+  uintptr_t a0, a1, b0, b1;
+  byte_range(a, a0, a1);
+  byte_range(b, b0, b1);
+  return a0 < b1 && b0 < a1;
+}
+
+// Whether two [tokens, heads, head_dim] tensors whose byte ranges overlap are different heads of the same token rows (parts of one
+// projection's output): same token stride, and the heads of both side by side within it.
+bool interleaves(const at::Tensor& a, const at::Tensor& b) {
+  if (a.element_size() != b.element_size() || a.stride(0) != b.stride(0) || a.stride(0) <= 0 || a.stride(1) < 0 || b.stride(1) < 0) return false;
+  const int64_t row = a.stride(0) * (int64_t)a.element_size();
+  auto span = [](const at::Tensor& t) { return ((t.size(1) - 1) * t.stride(1) + t.size(2)) * (int64_t)t.element_size(); };
+  const int64_t gap = (int64_t)((uintptr_t)b.data_ptr() - (uintptr_t)a.data_ptr());
+  const int64_t at = ((gap % row) + row) % row;  // where b's token rows start in a's
+  return at >= span(a) && at + span(b) <= row;
+}
+
+// rotary(query, key or None, positions, inv_freq, interleaved, attention_factor, inverse, out or None) -> (query, key or None)
+PyObject* rotary(PyObject*, PyObject* const* p, Py_ssize_t n) {
+  if (!expect("rotary", n, 8)) return nullptr;
+  return guarded([&]() -> PyObject* {
+    const at::Tensor& first = cuda_tensor(p[0], "query");
+    const int dev = device_index(first);
+    const bool has_key = p[1] != Py_None;
+    at::Tensor x[2] = {first, has_key ? on_device(cuda_tensor(p[1], "key"), dev, "key") : at::Tensor()}, y[2];
+    const at::Tensor& pos = on_device(cuda_tensor(p[2], "positions"), dev, "positions");
+    const at::Tensor& freq = on_device(cuda_tensor(p[3], "inv_freq"), dev, "inv_freq");
+    const int count = has_key ? 2 : 1;
+    for (int i = 0; i < count; ++i) {
+      TQ4_ASSERT(x[i].dim() == 3, "query and key must be [tokens, heads, head_dim]");
+      TQ4_ASSERT(x[i].size(0) == x[0].size(0) && x[i].size(2) == x[0].size(2) && x[i].scalar_type() == x[0].scalar_type(),
+                 "query and key must have the same tokens, head_dim and type");
+    }
+    const int64_t t = x[0].size(0), d = x[0].size(2), rot = 2 * freq.numel();
+    TQ4_ASSERT((pos.scalar_type() == at::kInt || pos.scalar_type() == at::kLong) && pos.dim() == 1 && pos.numel() == t && pos.is_contiguous(),
+               "positions must be contiguous int32 or int64 [tokens]");
+    TQ4_ASSERT((freq.scalar_type() == at::kFloat || freq.scalar_type() == at::kDouble) && freq.dim() == 1 && freq.is_contiguous(),
+               "inv_freq must be contiguous float32 or float64 [rotary_dim / 2]");
+    TQ4_ASSERT(rot > 0 && rot <= d, "inv_freq must have between 1 and head_dim / 2 entries");
+    const int dt = dtype_code(x[0].scalar_type());
+    const float factor = (float)as_double(p[5]);
+    const int interleaved = truth(p[4]), inverse = truth(p[6]);
+    PyObject* out[2] = {Py_None, Py_None};
+    if (p[7] != Py_None) {
+      TQ4_ASSERT(PyTuple_Check(p[7]) && PyTuple_GET_SIZE(p[7]) == 2, "out must be a pair (query, key)");
+      for (int i = 0; i < 2; ++i) out[i] = PyTuple_GET_ITEM(p[7], i);
+    }
+    Launch launch(dev);
+    for (int i = 0; i < count; ++i) {
+      if (out[i] == Py_None) {
+        x[i] = inner_contiguous(x[i]);
+        y[i] = at::empty(x[i].sizes(), x[i].options().requires_grad(false));
+        continue;
+      }
+      y[i] = on_device(cuda_tensor(out[i], "out"), dev, "out");
+      TQ4_ASSERT(y[i].sizes() == x[i].sizes() && y[i].scalar_type() == x[i].scalar_type() && (d < 2 || y[i].stride(2) == 1),
+                 "out must have the input's shape and type, and contiguous rows");
+      const bool same = y[i].data_ptr() == x[i].data_ptr() && y[i].strides() == x[i].strides();
+      TQ4_ASSERT(same || !overlap(y[i], x[i]), "an output must be its input or not overlap it");
+      x[i] = inner_contiguous(x[i]);
+    }
+    for (int i = 0; i < count; ++i) {
+      TQ4_ASSERT(y[i].numel() == 0 || ((y[i].size(0) < 2 || y[i].stride(0) != 0) && (y[i].size(1) < 2 || y[i].stride(1) != 0)),
+                 "an output may not be expanded");
+      TQ4_ASSERT(count < 2 || !overlap(y[i], x[1 - i]) || interleaves(y[i], x[1 - i]), "an output may not overlap the other input");
+    }
+    TQ4_ASSERT(count < 2 || !overlap(y[0], y[1]) || interleaves(y[0], y[1]), "the outputs may not overlap");
+    int64_t xs[2][2] = {}, ys[2][2] = {};
+    for (int i = 0; i < count; ++i)
+      for (int k = 0; k < 2; ++k) {
+        xs[i][k] = x[i].stride(k);
+        ys[i][k] = y[i].stride(k);
+      }
+    int st;
+    {
+      const NoGil no_gil;
+      st = tq4_rotary(x[0].data_ptr(), has_key ? x[1].data_ptr() : nullptr, dt, t, (int)x[0].size(1), has_key ? (int)x[1].size(1) : 0, (int)d,
+                      xs[0], xs[1], pos.data_ptr(), pos.scalar_type() == at::kLong, freq.data_ptr(), freq.scalar_type() == at::kDouble,
+                      (int)rot, interleaved, factor, inverse, y[0].data_ptr(), has_key ? y[1].data_ptr() : nullptr, ys[0], ys[1],
+                      launch.stream);
+    }
+    check(st, "tq4_rotary");
+    PyObject* pair = PyTuple_New(2);
+    if (!pair) throw PyError{};
+    for (int i = 0; i < 2; ++i) {
+      PyObject* o = i >= count ? Py_None : out[i];
+      if (i < count && o == Py_None) {
+        o = THPVariable_Wrap(std::move(y[i]));
+      } else {
+        Py_INCREF(o);
+      }
+      PyTuple_SET_ITEM(pair, i, o);
+    }
+    return pair;
+  });
+}
+
+// The caches of a call's layers: one [blocks, block_size, bytes] tensor, or a sequence of tensors that are alike.
+struct LayerCaches {
+  std::vector<uint8_t*> at;
+  std::vector<at::Tensor> held;  // (kept until the launch: the sequence may change in another thread meanwhile)
+  int dev = -1;
+  LayerCaches(PyObject* o) {
+    auto add = [&](PyObject* item) {
+      const at::Tensor& t = cuda_tensor(item, "kv_caches");
+      TQ4_ASSERT(t.scalar_type() == at::kByte && t.dim() == 3 && t.stride(2) == 1, "a cache must be uint8 [blocks, block_size, bytes] with contiguous rows");
+      if (held.empty()) dev = device_index(t);
+      else TQ4_ASSERT(t.get_device() == dev && t.sizes() == held[0].sizes() && t.strides() == held[0].strides(), "the layers' caches must be alike");
+      held.push_back(t);
+      at.push_back((uint8_t*)t.data_ptr());
+    };
+    if (THPVariable_Check(o)) {
+      add(o);
+    } else {
+      struct Held {
+        PyObject* o;
+        ~Held() { Py_XDECREF(o); }
+      } seq{PySequence_Tuple(o)};
+      if (!seq.o) throw PyError{};
+      for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(seq.o); ++i) add(PyTuple_GET_ITEM(seq.o, i));
+    }
+    TQ4_ASSERT(!held.empty(), "kv_caches must hold a cache");
+    std::vector<uint8_t*> sorted(at);
+    std::sort(sorted.begin(), sorted.end());
+    TQ4_ASSERT(std::adjacent_find(sorted.begin(), sorted.end()) == sorted.end(), "a cache may be in kv_caches once only");
+  }
+  const at::Tensor& first() const { return held[0]; }
+};
+
+// copy_blocks(kv_caches, block_mapping, num_kv_heads, head_dim)
+PyObject* copy_blocks(PyObject*, PyObject* const* p, Py_ssize_t n) {
+  if (!expect("copy_blocks", n, 4)) return nullptr;
+  return guarded([&]() -> PyObject* {
+    const LayerCaches caches(p[0]);
+    const at::Tensor& c = caches.first();
+    const at::Tensor& map = on_device(cuda_tensor(p[1], "block_mapping"), caches.dev, "block_mapping");
+    TQ4_ASSERT((map.scalar_type() == at::kInt || map.scalar_type() == at::kLong) && map.dim() == 2 && map.size(1) == 2 && map.is_contiguous(),
+               "block_mapping must be contiguous int32 or int64 [pairs, 2]");
+    const int64_t hkv = as_int(p[2]), d = as_int(p[3]);
+    Launch launch(caches.dev);
+    const size_t need = tq4_copy_blocks_workspace_bytes(map.size(0), c.size(0));
+    at::Tensor ws;
+    if (need) ws = workspace_of(caches.dev, launch.stream, (int64_t)need);
+    int* flag = (int*)flag_of(caches.dev).data_ptr();
+    int st;
+    {
+      const NoGil no_gil;
+      st = tq4_copy_blocks(caches.at.data(), (int)caches.at.size(), c.size(0), (int)c.size(1), c.stride(0), c.stride(1), (int)hkv, (int)d,
+                           map.data_ptr(), map.scalar_type() == at::kLong, map.size(0), need ? ws.data_ptr() : nullptr, need, flag,
+                           launch.stream);
+    }
+    check(st, "tq4_copy_blocks");
+    Py_RETURN_NONE;
+  });
+}
+
+// compact_rows(kv_caches, block_table, starts, keep, keep_lens, num_kv_heads, head_dim, seq_lens_out or None)
+PyObject* compact_rows(PyObject*, PyObject* const* p, Py_ssize_t n) {
+  if (!expect("compact_rows", n, 8)) return nullptr;
+  return guarded([&]() -> PyObject* {
+    const LayerCaches caches(p[0]);
+    const at::Tensor& c = caches.first();
+    auto input = [&](int i, const char* name) -> const at::Tensor& { return on_device(cuda_tensor(p[i], name), caches.dev, name); };
+    const at::Tensor &bt = input(1, "block_table"), &starts = input(2, "starts"), &keep = input(3, "keep"), &lens = input(4, "keep_lens");
+    const int64_t hkv = as_int(p[5]), d = as_int(p[6]);
+    auto list = [&](const at::Tensor& t, const char* msg) {
+      TQ4_ASSERT(t.scalar_type() == at::kInt && t.dim() == 1 && t.is_contiguous() && t.numel() == keep.size(0), msg);
+    };
+    TQ4_ASSERT(keep.scalar_type() == at::kInt && keep.dim() == 2 && (keep.size(1) < 2 || keep.stride(1) == 1),
+               "keep must be int32 [sequences, places] with contiguous rows");
+    TQ4_ASSERT(bt.scalar_type() == at::kInt && bt.dim() == 2 && bt.size(0) >= keep.size(0) && (bt.size(1) < 2 || bt.stride(1) == 1),
+               "block_table must be int32 [sequences, blocks] with contiguous rows");
+    list(starts, "starts must be contiguous int32 [sequences]");
+    list(lens, "keep_lens must be contiguous int32 [sequences]");
+    int32_t* lens_out = nullptr;
+    if (p[7] != Py_None) {
+      const at::Tensor& o = input(7, "seq_lens_out");
+      list(o, "seq_lens_out must be contiguous int32 [sequences]");
+      TQ4_ASSERT(!overlap(o, starts) && !overlap(o, lens) && !overlap(o, keep) && !overlap(o, bt), "seq_lens_out may not overlap an input");
+      lens_out = (int32_t*)o.data_ptr();
+    }
+    TQ4_ASSERT(keep.size(1) <= 0x7fffffff, "keep has too many places");
+    Launch launch(caches.dev);
+    const size_t need = tq4_compact_rows_workspace_bytes((int)caches.at.size(), (int)keep.size(0), (int)keep.size(1), (int)hkv, (int)d);
+    at::Tensor ws;
+    if (need) ws = workspace_of(caches.dev, launch.stream, (int64_t)need);
+    int* flag = (int*)flag_of(caches.dev).data_ptr();
+    int st;
+    {
+      const NoGil no_gil;
+      st = tq4_compact_rows(caches.at.data(), (int)caches.at.size(), c.size(0), (int)c.size(1), c.stride(0), c.stride(1), (int)hkv, (int)d,
+                            (const int32_t*)bt.data_ptr(), bt.stride(0), bt.size(1), (int)keep.size(0), (const int32_t*)starts.data_ptr(),
+                            (const int32_t*)keep.data_ptr(), keep.stride(0), (int)keep.size(1), (const int32_t*)lens.data_ptr(), lens_out,
+                            need ? ws.data_ptr() : nullptr, need, flag, launch.stream);
+    }
+    check(st, "tq4_compact_rows");
+    Py_RETURN_NONE;
+  });
+}
+
 // error_flag(device_index) -> the device's int32 flag tensor
 PyObject* error_flag(PyObject*, PyObject* const* p, Py_ssize_t n) {
   if (!expect("error_flag", n, 1)) return nullptr;
@@ -619,6 +950,11 @@ PyMethodDef kMethods[] = {
     {"append_rows", (PyCFunction)(void (*)(void))append_rows, METH_FASTCALL, "Compress K and V into token rows of a batch."},
     {"cache_update", (PyCFunction)(void (*)(void))cache_update, METH_FASTCALL, "Compress, store and reconstruct an update."},
     {"cache_step", (PyCFunction)(void (*)(void))cache_step, METH_FASTCALL, "An update by a plan."},
+    {"tree_attention", (PyCFunction)(void (*)(void))tree_attention, METH_FASTCALL, "Attention of trees of drafted tokens."},
+    {"tree_mask", (PyCFunction)(void (*)(void))tree_mask, METH_FASTCALL, "Masks of trees of drafted tokens."},
+    {"rotary", (PyCFunction)(void (*)(void))rotary, METH_FASTCALL, "Rotary positions of queries and keys."},
+    {"copy_blocks", (PyCFunction)(void (*)(void))copy_blocks, METH_FASTCALL, "Copy pages in the caches of all layers."},
+    {"compact_rows", (PyCFunction)(void (*)(void))compact_rows, METH_FASTCALL, "Move the token rows that stay together."},
     {"error_flag", (PyCFunction)(void (*)(void))error_flag, METH_FASTCALL, "Device error flag."},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_tq4_host", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};

@@ -422,14 +422,17 @@ struct Bars {
   uint64_t drain;                 // a dead CTA's last MMA complete
 };
 
-template <int D, bool FAST>
+// TREE: rows are drafts that see the keys in front of their sequence's drafts and, of those, what a.tree_mask says.  A sequence whose
+// rows fill one row block only has its tiles dealt to both blocks in turn, as two streams with the same queries: their tensor
+// work and softmax overlap as those of two row blocks do, and the second stream is folded into the first at the end.
+template <int D, bool FAST, bool TREE>
 __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(const AttnArgs a, const PrefillArgs pa) {
   using C = Cfg<D>;
   constexpr int NBLK = C::NBLK, TPR = C::TPR, CPT = C::CPT, DPT = C::DPT, NC = C::NC, NKB = C::NKB, NVB = C::NVB, NIT = C::NIT;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   __shared__ __align__(8) Bars s_bars;
   __shared__ uint32_t s_tmem;
-  __shared__ int s_info[5];      // sequence, first row and rows of the CTA; end of the sequence's rows and its length
+  __shared__ int s_info[6];      // sequence, first row and rows of the CTA; end of the sequence's rows and its length; their start
   __shared__ float s_cent[2][16];  // scaled centroids of K and V
   __shared__ int s_dead, s_bad;  // a wait gave up / some page id is out of range
   const AttnShape& sh = a.sh;
@@ -472,6 +475,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(const AttnArgs 
         if (lane == w) {
           s_info[3] = q_end;
           s_info[4] = seq_len;
+          if (TREE) s_info[5] = q0;
         }
       }
       acc += __shfl_sync(0xffffffffu, incl, 31);
@@ -537,7 +541,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(const AttnArgs 
   // ---- row of a softmax thread (half a row at head_dim 256), and its raw query on the way -------------------
   const int blk = NBLK == 2 ? (warp >> 2) & 1 : 0, part = NBLK == 2 ? 0 : (warp >> 2) & 1;
   const int m = 32 * (warp & 3) + lane, my_r = m / G, my_g = m - my_r * G;
-  const int lrow = blk * RB + my_r;                       // row within the CTA
+  const bool streams = TREE && NBLK == 2 && nrows <= RB;  // both blocks have the same rows, and every other tile
+  const int lrow = (streams ? 0 : blk * RB) + my_r;       // row within the CTA
   const bool live = warp < kSmx / 32 && my_r < RB && lrow < nrows;
   const int head = kvh * G + my_g, row = row0 + (live ? lrow : 0);
   const int es = a.q_dtype == TQ4_F32 ? 4 : 2;
@@ -579,17 +584,23 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(const AttnArgs 
 
   PF_STAMP(tid == 0 ? 0 : -1, 0, 5);
   // ---- keys the CTA needs: rows are in query order, their visible ranges move forward with them -----------
-  const int q_end = s_info[3], len = clamp_seq_len(a, max(0, s_info[4]));
+  const int q_end = s_info[3], len = clamp_seq_len<TREE>(a, max(0, s_info[4]));
   auto row_keys = [&](int row, int& lo, int& hi) {  // visible keys of row `row` of the call
     const int pos = len - (q_end - row);
     hi = max(0, min(a.causal ? pos + 1 : len, len));
     lo = min(a.sliding_window > 0 ? max(0, pos + 1 - a.sliding_window) : 0, hi);
   };
   int blk_lo, blk_hi, t_first = 0, n_tiles = 0;
+  const int held = TREE ? len - (q_end - s_info[5]) : 0;  // keys in front of the drafts
   {
-    int x;
-    row_keys(row0, blk_lo, x);
-    row_keys(row0 + nrows - 1, x, blk_hi);
+    if (TREE) {  // (a row's position is held - 1 or later)
+      blk_lo = a.sliding_window > 0 ? min(max(0, held - a.sliding_window), len) : 0;
+      blk_hi = len;
+    } else {
+      int x;
+      row_keys(row0, blk_lo, x);
+      row_keys(row0 + nrows - 1, x, blk_hi);
+    }
     if (blk_hi > blk_lo) {
       t_first = blk_lo / kBN * kBN;
       n_tiles = (blk_hi - t_first + kBN - 1) / kBN;
@@ -598,7 +609,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(const AttnArgs 
       n_tiles = max(0, min(per, n_tiles - (int)blockIdx.z * per));
     }
   }
-  const int n_blk = nrows > RB ? NBLK : 1;  // row blocks in use
+  const int n_blk = streams ? (n_tiles > 1 ? 2 : 1) : nrows > RB ? NBLK : 1;  // row blocks in use
 
   if (warp == kIssueWarp) {
     // ================= issuing thread =================
@@ -637,7 +648,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(const AttnArgs 
           constexpr uint32_t N = C::kChunks == 1 ? D : 64;
           const uint32_t idesc = C::idesc(N, unrot);
           const uint32_t hi = unrot ? uhi : img, lo = unrot ? ulo : img + C::kImg / 2;
-          for (int b = 0; b < n_blk; ++b) {
+          for (int b = 0; b < (streams && unrot ? 1 : n_blk); ++b) {
             const uint32_t tb = tmem + b * C::kBlkCols, d = tb + C::kColO + 64 * ch;
 #pragma unroll 1
             for (int s = 0; s < D / 16; ++s) {
@@ -679,15 +690,15 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(const AttnArgs 
         }
         mma_commit(bar(s_bars.sready[NBLK == 1 ? j & 1 : b]));
       };
-      auto issue_pv = [&](int b, int j) {  // O += P V~ of tile j
+      auto issue_pv = [&](int b, int j, int n) {  // O += P V~ of tile j, the block's tile n
         const uint32_t tb = tmem + b * C::kBlkCols, p = tb + C::kColS + (NBLK == 1 ? 64 * (j & 1) : 0);
         const uint64_t dv0 = d_v + (uint64_t)(((j % NVB) * C::kKvBuf) >> 4);
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
           const uint64_t dv = dv0 + (uint64_t)((2048 * s) >> 4);
           const uint32_t ph = p + 16 * s;
-          if (!FAST) mma_ta(tb + C::kColO, ph + 8, dv, idO, j > 0 || s > 0);
-          mma_ta(tb + C::kColO, ph, dv, idO, !FAST || j > 0 || s > 0);
+          if (!FAST) mma_ta(tb + C::kColO, ph + 8, dv, idO, n > 0 || s > 0);
+          mma_ta(tb + C::kColO, ph, dv, idO, !FAST || n > 0 || s > 0);
         }
       };
       auto wait_k = [&](int j) { ok = ok && bar_wait(bar(s_bars.kready[j % NKB]), (uint32_t)((j / NKB) & 1), dead); };
@@ -698,11 +709,35 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(const AttnArgs 
       wait_k(0);
       if (ok) {
         fence_after();
-        for (int b = 0; b < n_blk; ++b) issue_s(b, 0);
+        for (int b = 0; b < (streams ? 1 : n_blk); ++b) issue_s(b, 0);
         mma_commit(bar(s_bars.kfree[0]));
       }
+      if (streams && n_tiles > 1) {
+        wait_k(1);
+        if (ok) {
+          fence_after();
+          issue_s(1, 1);
+          mma_commit(bar(s_bars.kfree[1]));
+        }
+      }
       for (int j = 0; j < n_tiles && ok; ++j) {
-        if (NBLK == 1) {  // the next tile's scores go into the other S while this tile is in its softmax
+        if (streams) {  // tile j is block j % 2's
+          const int b = j & 1;
+          wait_v(j);
+          if (j == n_tiles - 1 && unrotate && ok) load_chunk(0, true);
+          wait_p(b, j >> 1);
+          if (!ok) break;
+          fence_after();
+          issue_pv(b, j, j >> 1);
+          mma_commit(bar(s_bars.vfree[b]));
+          if (j + 2 < n_tiles) {
+            wait_k(j + 2);
+            if (!ok) break;
+            fence_after();
+            issue_s(b, j + 2);
+            mma_commit(bar(s_bars.kfree[b]));
+          }
+        } else if (NBLK == 1) {  // the next tile's scores go into the other S while this tile is in its softmax
           if (j + 1 < n_tiles) {
             wait_k(j + 1);
             if (!ok) break;
@@ -721,7 +756,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(const AttnArgs 
           }
           if (!ok) break;
           fence_after();
-          issue_pv(0, j);
+          issue_pv(0, j, j);
           mma_commit(bar(s_bars.vfree[j % NVB]));
           mma_commit(bar(s_bars.pvd));
         } else {  // the blocks take turns: while one is in its softmax the other has the tensor pipe
@@ -734,7 +769,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(const AttnArgs 
             PF_STAMP(3, j, 2 * b);
             if (!ok) break;
             fence_after();
-            issue_pv(b, j);
+            issue_pv(b, j, j);
             if (b == n_blk - 1) mma_commit(bar(s_bars.vfree[j % NVB]));
             if (j + 1 < n_tiles) {
               if (b == 0) {
@@ -958,7 +993,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(const AttnArgs 
       if (lane == 0) bar_arrive(bar(b));
     };
     bool ok = true;
-    const bool use = n_tiles > 0 && blk < n_blk;  // (uniform per warp)
+    bool use = n_tiles > 0 && blk < n_blk, mine = live;  // (`use`: uniform per warp)
     // the raw queries were asked for, whether this part has keys (then the wait is below) or not.  (One wait for both
     // here, in front of the branch, lengthens a tile by 2 %: 4977 against 4863 us at 8 x 2048 rows on 8192 cached.)
     if (q_staged && n_tiles == 0) bar_wait_own(bar(s_bars.qraw), 0u, dead);
@@ -1065,16 +1100,36 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(const AttnArgs 
     PF_STAMP(tid == 0 ? 0 : -1, 0, 6);
     // ---- the tile loop --------------------------------------------------------------------------------
     int kv_lo = 0, kv_hi = 0x7fffffff;  // (a row that is not there: zeros, nothing to mask)
-    if (live) row_keys(row, kv_lo, kv_hi);
+    const uint32_t* drafts = nullptr;   // TREE: the row's mask
+    if (TREE) {
+      if (live) {
+        drafts = reinterpret_cast<const uint32_t*>(a.tree_mask) + (int64_t)row * a.tree_stride;
+        kv_hi = max(held, 0);
+        if (a.sliding_window > 0) {
+          int n = 0;
+          for (int w = 0; w < a.tree_words; ++w) n += __popc(__ldg(drafts + w));
+          kv_lo = min(max(0, held + n - a.sliding_window), kv_hi);
+        }
+      }
+    } else if (live) {
+      row_keys(row, kv_lo, kv_hi);
+    }
+    // 32 bits of the row's mask from draft `k` on
+    auto draft_bits = [&](int k) -> uint32_t {
+      auto word = [&](int w) -> uint32_t { return (unsigned)w < (unsigned)a.tree_words ? __ldg(drafts + w) : 0u; };
+      const int w = k >> 5;  // (k may be negative)
+      return __funnelshift_r(word(w), word(w + 1), k & 31);
+    };
     float m_run = -CUDART_INF_F, l_run = 0.f;
     const int role = tid == 0 ? 0 : tid == 128 ? 1 : -1;  // (time stamps)
     (void)role;
     if (use) {
-      for (int j = 0; j < n_tiles && ok; ++j) {
+      for (int j = streams ? blk : 0; j < n_tiles && ok; j += streams ? 2 : 1) {
+        const int nth = streams ? j >> 1 : j;  // of the block's tiles
         PF_STAMP(role, j, 0);
         const int t0 = t_first + j * kBN + part * CPT;  // first token of this thread's columns
         const int sb = NBLK == 1 ? j & 1 : blk;
-        ok = __all_sync(0xffffffffu, bar_wait(bar(s_bars.sready[sb]), (uint32_t)((NBLK == 1 ? j >> 1 : j) & 1), dead));
+        ok = __all_sync(0xffffffffu, bar_wait(bar(s_bars.sready[sb]), (uint32_t)((NBLK == 1 ? j >> 1 : nth) & 1), dead));
         if (!ok) break;
         PF_STAMP(role, j, 1);
         fence_after();
@@ -1104,6 +1159,10 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(const AttnArgs 
             for (int w = 0; w < CPT / 32; ++w) {
               const int l = min(max(lo - 32 * w, 0), 32), h = min(max(hi - 32 * w, 0), 32);
               vis[w] = h > l ? (0xFFFFFFFFu >> (32 - (h - l))) << l : 0u;
+              if (TREE && live) {  // (drafts of the sequence only)
+                const int k = t0 + 32 * w - held, n = min(max(len - (t0 + 32 * w), 0), 32);
+                if (n > 0 && k > -32) vis[w] |= draft_bits(k) & (0xFFFFFFFFu >> (32 - n));
+              }
               if (*(volatile int*)&s_bad)
                 for (int i = 0; i < 32; ++i)
                   if (ns[32 * w + i] == kHidden) vis[w] &= ~(1u << i);
@@ -1196,7 +1255,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(const AttnArgs 
           const float alpha = bump ? (m_run == -CUDART_INF_F ? 0.f : ex2_approx(m_run - mt)) : 1.f;
           if (bump) m_run = mt;
           l_run *= alpha;
-          if (j > 0) {  // O: no MMA is working on it
+          if (nth > 0) {  // O: no MMA is working on it
             if (NBLK == 1) {
               ok = __all_sync(0xffffffffu, bar_wait(bar(s_bars.pvd), (uint32_t)((j - 1) & 1), dead));
               fence_after();
@@ -1230,6 +1289,51 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(const AttnArgs 
       fence_after();
       have = ok && l_run > 0.f;
     }
+    if (streams && n_blk == 2) {  // (uniform) the second stream's sums into the first's
+      float* s_o = reinterpret_cast<float*>(sm + C::kOffK);  // [128][D] where K~ and V~ were, 16-byte pieces of a row rotated by it
+      static_assert(!TREE || NBLK == 1 || C::kOffV + NVB * C::kKvBuf >= 128u * D * 4, "room for a block's sums");
+      float2* s_ml = reinterpret_cast<float2*>(sm + C::kOffNorm);
+      auto piece = [&](int p) { return reinterpret_cast<float4*>(s_o + m * D + 4 * ((p + m) % (D / 4))); };
+      if (blk == 1) {
+        s_ml[m] = make_float2(ok ? m_run : -CUDART_INF_F, ok ? l_run : 0.f);
+#pragma unroll 1
+        for (int q = 0; q < DPT / 16; ++q) {
+          uint32_t o[16];
+          tmem_ld16_async(tb + C::kColO + 16 * q, o);
+          tmem_ld16_wait(o);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            *piece(4 * q + i) = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]), __uint_as_float(o[4 * i + 2]),
+                                            __uint_as_float(o[4 * i + 3]));
+        }
+      }
+      asm volatile("bar.sync 1, %0;" ::"n"(kSmx) : "memory");
+      if (blk == 0) {
+        const float2 other = s_ml[m];
+        const float top = fmaxf(m_run, other.x), ref = top == -CUDART_INF_F ? 0.f : top;
+        const float f0 = ex2_approx(m_run - ref), f1 = ex2_approx(other.x - ref);
+        m_run = top;
+        l_run = l_run * f0 + other.y * f1;
+        have = ok && l_run > 0.f;
+#pragma unroll 1
+        for (int q = 0; q < DPT / 16; ++q) {
+          uint32_t o[16];
+          tmem_ld16_async(tb + C::kColO + 16 * q, o);
+          tmem_ld16_wait(o);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float4 y = *piece(4 * q + i);
+            o[4 * i] = __float_as_uint(__uint_as_float(o[4 * i]) * f0 + y.x * f1);
+            o[4 * i + 1] = __float_as_uint(__uint_as_float(o[4 * i + 1]) * f0 + y.y * f1);
+            o[4 * i + 2] = __float_as_uint(__uint_as_float(o[4 * i + 2]) * f0 + y.z * f1);
+            o[4 * i + 3] = __float_as_uint(__uint_as_float(o[4 * i + 3]) * f0 + y.w * f1);
+          }
+          tmem_st16(tb + C::kColO + 16 * q, o);
+        }
+        tmem_st_wait();
+      }
+    }
+    if (streams && blk == 1) use = mine = have = false;  // from here on a block without rows
     const float inv = have ? 1.f / (a.lut_scale_v * l_run) : 0.f;
     const float lse = have ? (m_run + lg2_approx(l_run)) * 0.6931471805599453f : -CUDART_INF_F;
     const bool out_vec = (uintptr_t)a.out % 16 == 0 && a.out_token_stride % 8 == 0 && a.out_head_stride % 8 == 0;
@@ -1242,15 +1346,15 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(const AttnArgs 
       for (int c = 0; c < DPT / 32; ++c) {
         uint32_t v[32];
         if (use && ok) tmem_ld32(tb + C::kColO + part * DPT + 32 * c, v);
-        if (live) {
+        if (mine) {
           float y[32];
 #pragma unroll
           for (int e = 0; e < 32; ++e) y[e] = have ? __uint_as_float(v[e]) * inv : 0.f;
           store32(dst, dt, oi + part * DPT + 32 * c, out_vec, y);
         }
       }
-      if (live && part == 0 && pa.to_parts) pa.part_m[vec] = lse;
-      else if (live && part == 0 && a.lse_out) a.lse_out[(int64_t)row * sh.Hq + head] = lse;
+      if (mine && part == 0 && pa.to_parts) pa.part_m[vec] = lse;
+      else if (mine && part == 0 && a.lse_out) a.lse_out[(int64_t)row * sh.Hq + head] = lse;
     } else {
       float isc = 0.f;
       if (use) {
@@ -1293,7 +1397,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(const AttnArgs 
       for (int c = 0; c < DPT / 32; ++c) {
         uint32_t v[32];
         if (use && ok) tmem_ld32(tb + C::kColO + part * DPT + 32 * c, v);
-        if (live) {
+        if (mine) {
           float y[32];
 #pragma unroll
           for (int e = 0; e < 32; ++e) y[e] = f != 0.f ? __uint_as_float(v[e]) * f : 0.f;
@@ -1305,7 +1409,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(const AttnArgs 
         __syncwarp();
         constexpr int PCS = DPT / 8;  // 16-byte pieces of a thread's part of a row
         const unsigned char* rows = sm + C::kOffQlo + (blk * 128 + 32 * (warp & 3)) * C::kQPitch + part * DPT * 2;
-        const int64_t to = live ? oi : -1;
+        const int64_t to = mine ? oi : -1;
 #pragma unroll 4
         for (int i = lane; i < 32 * PCS; i += 32) {
           const int r = i / PCS, pc = i - r * PCS;
@@ -1314,7 +1418,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(const AttnArgs 
             *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(a.out) + at + 8 * pc) = *reinterpret_cast<const uint4*>(rows + r * C::kQPitch + 16 * pc);
         }
       }
-      if (live && part == 0 && a.lse_out) a.lse_out[(int64_t)row * sh.Hq + head] = lse;
+      if (mine && part == 0 && a.lse_out) a.lse_out[(int64_t)row * sh.Hq + head] = lse;
     }
   }
   fence_before();
@@ -1326,7 +1430,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(const AttnArgs 
   }
 }
 
-template <int D, bool FAST>
+template <int D, bool FAST, bool TREE>
 int launch_t(const AttnArgs& a, PrefillArgs pa, cudaStream_t st) {
   using C = Cfg<D>;
   constexpr int smem = (int)C::kSmem + 1024;
@@ -1334,7 +1438,7 @@ int launch_t(const AttnArgs& a, PrefillArgs pa, cudaStream_t st) {
   static_assert(2 * smem > 227 * 1024 || D < 128, "one CTA per SM: it allocates the whole tensor memory");
   // (head_dim 64 and 96 need less: ask for more than half of the SM so that only one CTA fits)
   constexpr int ask = smem > 120 * 1024 ? smem : 120 * 1024;
-  if (!ensure_dynamic_smem<prefill_tc_kernel<D, FAST>>(ask)) return TQ4_ERR_CUDA;
+  if (!ensure_dynamic_smem<prefill_tc_kernel<D, FAST, TREE>>(ask)) return TQ4_ERR_CUDA;
   const int per_cta = C::NBLK * (128 / a.sh.G);
   const unsigned blocks = (unsigned)((a.sh.rows + per_cta - 1) / per_cta + a.sh.num_seqs);  // upper bound
   // More CTAs than fit at once: the KV heads run fastest, so that all heads of a sequence's last rows (the longest) start before any of
@@ -1347,21 +1451,23 @@ int launch_t(const AttnArgs& a, PrefillArgs pa, cudaStream_t st) {
   const int64_t grid = (int64_t)blocks * a.sh.Hkv;
   if (grid > 0x7fffffff) return TQ4_ERR_UNSUPPORTED;
   pa.heads_first = grid * pa.splits > sm_count();
-  if (launch_kernel(prefill_tc_kernel<D, FAST>, dim3((unsigned)grid, 1, (unsigned)pa.splits), dim3(kThreads), (size_t)ask, st, true, a,
+  if (launch_kernel(prefill_tc_kernel<D, FAST, TREE>, dim3((unsigned)grid, 1, (unsigned)pa.splits), dim3(kThreads), (size_t)ask, st, true, a,
                     pa) != cudaSuccess)
     return TQ4_ERR_CUDA;
   TQ4_CHECK_LAUNCH();
   return TQ4_OK;
 }
 
-template <int D>
+template <int D, bool TREE = false>
 int launch_d(const AttnArgs& a, const PrefillArgs& pa, cudaStream_t st, bool fast, uint8_t* image) {
   constexpr int n = D * ((D + 63) / 64) * 8;
   // first kernel of the prefill part: a plain launch (what the caller and the streaming part wrote is complete)
   if (launch_kernel(pi_image_kernel<D>, dim3((n + 255) / 256), dim3(256), 0, st, false, a.rotation, image) != cudaSuccess)
     return TQ4_ERR_CUDA;
   TQ4_CHECK_LAUNCH();
-  return fast ? launch_t<D, true>(a, pa, st) : launch_t<D, false>(a, pa, st);
+  if constexpr (!TREE)
+    if (fast) return launch_t<D, true, false>(a, pa, st);
+  return launch_t<D, false, TREE>(a, pa, st);
 }
 
 size_t image_bytes(int D) { return (size_t)2 * ((D + 63) / 64) * D * 128; }
@@ -1398,6 +1504,29 @@ int launch_prefill_tc(const AttnArgs& a, cudaStream_t st, bool fast, int min_row
     case 96: return launch_d<96>(a, pa, st, fast, image);
     case 128: return launch_d<128>(a, pa, st, fast, image);
     case 256: return launch_d<256>(a, pa, st, fast, image);
+  }
+  return TQ4_ERR_UNSUPPORTED;
+}
+
+// Key parts of a tree call.  A sequence has a CTA at least, whatever its rows.
+int tree_tc_splits(const AttnArgs& a, int64_t slots) {
+  const int per_cta = (a.sh.D == 256 ? 1 : 2) * (128 / a.sh.G);
+  const int64_t blocks = (a.sh.rows + per_cta - 1) / per_cta, ctas = (blocks > a.sh.num_seqs ? blocks : a.sh.num_seqs) * a.sh.Hkv;
+  int64_t s = sm_count() / (ctas > 0 ? ctas : 1);
+  const int64_t tiles = a.max_keys / kBN;
+  if (s > tiles / 4) s = tiles / 4;
+  if (s > 32) s = 32;
+  if (a.sh.rows > 0 && s > slots / a.sh.rows) s = slots / a.sh.rows;
+  return s < 1 ? 1 : (int)s;
+}
+
+int launch_tree_tc(const AttnArgs& a, cudaStream_t st, int splits, bool to_parts, uint8_t* image, float* part_o, float* part_m) {
+  const PrefillArgs pa{image, 1, splits, to_parts ? 1 : 0, part_o, part_m};
+  switch (a.sh.D) {
+    case 64: return launch_d<64, true>(a, pa, st, false, image);
+    case 96: return launch_d<96, true>(a, pa, st, false, image);
+    case 128: return launch_d<128, true>(a, pa, st, false, image);
+    case 256: return launch_d<256, true>(a, pa, st, false, image);
   }
   return TQ4_ERR_UNSUPPORTED;
 }

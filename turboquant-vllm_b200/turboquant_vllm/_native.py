@@ -31,6 +31,7 @@ F32, F16, BF16 = 0, 1, 2
 _DTYPE_CODE = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
 
 DEV_BAD_SLOT, DEV_BAD_BLOCK, DEV_TIMEOUT, DEV_WRITE_ORDER = 1, 2, 4, 8
+DEV_PAGE_CONFLICT, DEV_KEEP_ORDER, DEV_BAD_TREE = 16, 32, 128
 STATIC_SCRATCH_BYTES = 32 << 20
 
 # name -> (restype, argtypes); must list every symbol of include/tq4.h
@@ -86,6 +87,23 @@ _SIGNATURES = {
                                            c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int,
                                            c_void_p, c_int, c_void_p, c_float, c_int, c_int,
                                            c_void_p, c_int, c_int64, c_int64, c_int, c_void_p, c_void_p]),
+    "tq4_rotary": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int,
+                           c_void_p, c_int, c_int, c_int, c_float, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "tq4_tree_mask": (c_int, [c_void_p, c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "tq4_tree_attention_workspace_bytes": (c_size_t, [c_int64, c_int, c_int, c_int]),
+    "tq4_tree_attention": (c_int, [c_void_p, c_int, c_int64, c_int, c_int, c_int, c_int,
+                                   c_int64, c_int64, c_void_p, c_int64, c_int64, c_int64, c_int,
+                                   c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_int,
+                                   c_void_p, c_int, c_void_p, c_int, c_void_p, c_float, c_int,
+                                   c_void_p, c_int, c_int64, c_int64, c_void_p, c_int,
+                                   c_void_p, c_size_t, c_void_p, c_void_p]),
+    "tq4_copy_blocks_workspace_bytes": (c_size_t, [c_int64, c_int64]),
+    "tq4_copy_blocks": (c_int, [c_void_p, c_int, c_int64, c_int, c_int64, c_int64, c_int, c_int, c_void_p, c_int,
+                                c_int64, c_void_p, c_size_t, c_void_p, c_void_p]),
+    "tq4_compact_rows_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int]),
+    "tq4_compact_rows": (c_int, [c_void_p, c_int, c_int64, c_int, c_int64, c_int64, c_int, c_int, c_void_p,
+                                 c_int64, c_int64, c_int, c_void_p, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_void_p,
+                                 c_size_t, c_void_p, c_void_p]),
     "tq4_profile_start": (c_int, [c_int]),
     "tq4_profile_stop": (c_int, []),
     "tq4_profile_read": (c_int, [c_int, c_void_p, c_int]),
@@ -205,13 +223,17 @@ _DEV_BITS = ((DEV_BAD_SLOT, "slot_mapping entry outside the cache (TQ4_DEV_BAD_S
                              "block-table row (TQ4_DEV_BAD_BLOCK)"),
              (DEV_TIMEOUT, "a bounded device-side wait gave up (TQ4_DEV_TIMEOUT)"),
              (DEV_WRITE_ORDER, "a fused decode step wrote a token to a slot that is not the last position of "
-                               "its sequence (TQ4_DEV_WRITE_ORDER)"))
+                               "its sequence (TQ4_DEV_WRITE_ORDER)"),
+             (DEV_PAGE_CONFLICT, "a page was the destination of two copies, or of one and the source of another "
+                                 "(TQ4_DEV_PAGE_CONFLICT)"),
+             (DEV_KEEP_ORDER, "a list of rows to keep was not strictly increasing or longer than its row (TQ4_DEV_KEEP_ORDER)"),
+             (DEV_BAD_TREE, "a draft's parent was no earlier draft, or a draft lay behind the mask's last bit (TQ4_DEV_BAD_TREE)"))
 
 
 def describe_device_errors(flag: int) -> str:
     """Text for the TQ4_DEV_* bits a kernel OR-ed into the device error flag."""
     parts = [text for bit, text in _DEV_BITS if flag & bit]
-    rest = flag & ~(DEV_BAD_SLOT | DEV_BAD_BLOCK | DEV_TIMEOUT | DEV_WRITE_ORDER)
+    rest = flag & ~sum(bit for bit, _ in _DEV_BITS)
     if rest:
         parts.append(f"unknown bits {rest:#x}")
     return "; ".join(parts) if parts else "no error"

@@ -8,7 +8,9 @@ reference's Triton wrappers so existing callers and tests keep working:
 * ``fused_paged_tq4_decode``  (reference: src/turboquant_vllm/triton/fused_paged_tq4_attention.py:255-370)
 * ``fused_paged_tq4_int8_prefill`` (reference: src/turboquant_vllm/triton/fused_paged_tq4_int8_prefill.py:291-417)
 
-plus the fused cache write ``tq4_write_paged`` and the general ``paged_tq4_attention``.
+plus the fused cache write ``tq4_write_paged``, the general ``paged_tq4_attention``, and what a server that drafts
+several tokens a step needs around them: ``tq4_rotary``, ``tq4_tree_mask``, ``paged_tq4_tree_attention``,
+``tq4_compact_rows`` and ``tq4_copy_blocks``.
 Everything runs through the C ABI in ``include/tq4.h``; CPU tensors are rejected.
 """
 
@@ -476,3 +478,127 @@ def paged_tq4_attention_static(
     )
     nv.check(st, "paged_tq4_attention_static")
     return out
+
+
+# --------------------------------------------------------------------------------------
+# trees of drafted tokens
+# --------------------------------------------------------------------------------------
+def tq4_rotary(
+    query: torch.Tensor,
+    key: torch.Tensor | None,
+    positions: torch.Tensor,
+    inv_freq: torch.Tensor,
+    *,
+    interleaved: bool = False,
+    attention_factor: float = 1.0,
+    inverse: bool = False,
+    out: tuple[torch.Tensor, torch.Tensor | None] | None = None,
+) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """Rotary positions of ``query [T, Hq, D]`` and ``key [T, Hkv, D]`` in one launch, as the cache write wants its keys.
+
+    Frequency ``i`` of ``inv_freq`` (fp64 or fp32 ``[rotary_dim / 2]``, see :func:`turboquant_vllm.rotary.rotary_inv_freq`) turns
+    dimensions ``(i, i + rotary_dim / 2)`` of a head, or ``(2 i, 2 i + 1)`` when ``interleaved``, by ``positions[t] * inv_freq[i]``
+    (an exact product: no precision is lost far into a context) and scales them by ``attention_factor``; dimensions from
+    ``rotary_dim`` on are handed through.  ``inverse`` turns back, which is also the gradient of the turn.  ``positions``: int32 or
+    int64 ``[T]``; for a draft its depth behind the tokens held.  ``out=(q, k)``: results go there; an output may be its own input
+    (in place).  The rotation and the scaling are computed in fp32 and rounded once to the input's type.
+    """
+    return nv.host().rotary(query, key, positions, inv_freq, interleaved, attention_factor, inverse, out)
+
+
+def tq4_tree_mask(
+    parents: torch.Tensor, query_start_loc: torch.Tensor, max_nodes: int
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """Masks of trees of drafted tokens: ``(mask int32 [T, ceil(max_nodes / 32)], depth int32 [T])``.
+
+    ``parents`` int32 ``[T]``: for every draft the place, among its sequence's drafts, of the one that it continues (-1: the tokens
+    held); ``query_start_loc`` int32 ``[num_seqs + 1]``.  Bit ``k % 32`` of word ``k // 32`` of a row's mask is set where draft ``k``
+    is the row itself or one of its ancestors, whose number is its depth.  Made once a step, for all layers.
+    """
+    return nv.host().tree_mask(parents, query_start_loc, max_nodes)
+
+
+def tree_attention_workspace_bytes(max_query_rows: int, num_q_heads: int, num_kv_heads: int, head_dim: int) -> int:
+    """Bytes of scratch ``paged_tq4_tree_attention`` needs for up to ``max_query_rows`` rows."""
+    n = nv.lib().tq4_tree_attention_workspace_bytes(max_query_rows, num_q_heads, num_kv_heads, head_dim)
+    if n == 0:
+        raise ValueError(f"unsupported attention shape: Hq={num_q_heads}, Hkv={num_kv_heads}, D={head_dim}")
+    return int(n)
+
+
+def paged_tq4_tree_attention(
+    q: torch.Tensor,
+    kv_cache: torch.Tensor,
+    block_table: torch.Tensor,
+    seq_lens: torch.Tensor,
+    query_start_loc: torch.Tensor,
+    tree_mask: torch.Tensor,
+    k_centroids: torch.Tensor,
+    v_centroids: torch.Tensor,
+    rotation: torch.Tensor,
+    num_kv_heads: int,
+    block_size: int,
+    sm_scale: float | None = None,
+    *,
+    sliding_window: int | None = None,
+    out: torch.Tensor | None = None,
+    out_dtype: torch.dtype | None = None,
+    lse_out: torch.Tensor | None = None,
+    out_rotated: bool = False,
+    workspace: torch.Tensor | None = None,
+    max_seq_len: int | None = None,
+) -> torch.Tensor:
+    """Attention of trees of drafted tokens ``q [T, Hq, D]`` over the packed paged cache.
+
+    Sequence ``i`` drafts rows ``[query_start_loc[i], query_start_loc[i + 1])``, whose keys and values are in the cache already
+    (:func:`tq4_write_paged`), at the last positions of its ``seq_lens[i]``.  A row sees every key in front of the drafts, and of the
+    drafts those whose bits are set in its row of ``tree_mask`` (:func:`tq4_tree_mask`, or any other int32 ``[T, words]``).
+    ``sliding_window``: of the keys in front of the drafts, those within the window of the row's position, which is that of the last
+    of them plus the number of its set bits; the drafts are left to the mask.  A row that sees nothing gets zeros (``lse_out``: -inf).
+    The other arguments, and the precision, are those of :func:`paged_tq4_attention`.
+    """
+    return nv.host().tree_attention(
+        q, kv_cache, block_table, seq_lens, query_start_loc, tree_mask, k_centroids, v_centroids, rotation, num_kv_heads, block_size,
+        sm_scale, sliding_window, out, out_dtype, lse_out, out_rotated, workspace, max_seq_len)
+
+
+# --------------------------------------------------------------------------------------
+# moving what the cache holds
+# --------------------------------------------------------------------------------------
+def tq4_copy_blocks(
+    kv_caches: torch.Tensor | list[torch.Tensor] | tuple[torch.Tensor, ...],
+    block_mapping: torch.Tensor,
+    num_kv_heads: int,
+    head_dim: int,
+) -> None:
+    """Copy pages inside the caches ``(NB, BS, >= H*(D+8))`` of one or all layers, in one launch: a sequence is forked, a page that is
+    shared is about to be written.
+
+    ``block_mapping`` int32 or int64 ``[pairs, 2]``, on the device: ``(source, destination)``.  A page may be the destination of one
+    pair only, and not the source of another: where it is, the first of the pairs that write it counts, a pair that would read it is
+    not carried out, and the device's error flag says so (:func:`raise_on_device_errors`).  Padding behind a row's data is not touched.
+    """
+    nv.host().copy_blocks(kv_caches, block_mapping, num_kv_heads, head_dim)
+
+
+def tq4_compact_rows(
+    kv_caches: torch.Tensor | list[torch.Tensor] | tuple[torch.Tensor, ...],
+    block_table: torch.Tensor,
+    starts: torch.Tensor,
+    keep: torch.Tensor,
+    keep_lens: torch.Tensor,
+    num_kv_heads: int,
+    head_dim: int,
+    *,
+    seq_lens_out: torch.Tensor | None = None,
+) -> None:
+    """Move the token rows that stay together, in place, in the caches of one or all layers: the accepted path of a tree of drafts
+    (``starts``: the tokens held in front of it), or what an eviction leaves of a context (``starts``: the first position that it is
+    about).
+
+    For ``j < keep_lens[i]`` the row at position ``starts[i] + keep[i, j]`` of sequence ``i`` goes to ``starts[i] + j``; ``keep`` int32
+    ``[num_seqs, places]`` is strictly increasing in each row.  Rows behind the last one stay as they are, and so does a sequence whose
+    list is out of order or longer than its row (the device's error flag says so).  The pages from ``starts[i]`` on must be sequence
+    ``i``'s alone.  ``seq_lens_out`` int32 ``[num_seqs]`` gets ``starts + keep_lens``.
+    """
+    nv.host().compact_rows(kv_caches, block_table, starts, keep, keep_lens, num_kv_heads, head_dim, seq_lens_out)
