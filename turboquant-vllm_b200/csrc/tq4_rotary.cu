@@ -24,9 +24,11 @@ struct RotaryArgs {
   int64_t x_token_stride[2], x_head_stride[2], y_token_stride[2], y_head_stride[2];
   int heads[2];
   int64_t n_tokens;
-  int rot, per_head;  // rotary dimensions; items of a head (turned ones first, then those handed through)
+  int rot, items;     // rotary dimensions; items of a head (turned ones first, then those handed through)
   int turned;         // ... of which turned
-  int tokens;         // of a block
+  int per_head;       // items of a head in a block
+  int lanes;          // threads that share a token's item, each with every lanes-th head
+  int pass, tokens;   // tokens of a block at a time, and in all
   const void* positions;
   int positions_64;
   const void* inv_freq;
@@ -35,122 +37,181 @@ struct RotaryArgs {
   int inverse;
 };
 
+// V elements as they are in memory: words of two 16-bit values or one float, or a single element
 template <typename T, int V>
-struct alignas(V * sizeof(T) <= 16 ? V * sizeof(T) : 16) Chunk {
-  T v[V];
+struct alignas(V * sizeof(T)) Chunk {
+  static constexpr int kWords = V * sizeof(T) / 4;
+  uint32_t w[kWords];
 };
+template <>
+struct Chunk<__half, 1> { uint16_t w[1]; };
+template <>
+struct Chunk<__nv_bfloat16, 1> { uint16_t w[1]; };
 
-// V elements of one type are moved at a time.  An item is the two chunks whose elements make V pairs (half layout: V i and
-// rot / 2 + V i; interleaved: 2 V i and the one behind it), or one chunk of the dimensions that do not turn.
+__device__ __forceinline__ float2 unpack2(uint32_t w, __half) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+__device__ __forceinline__ float2 unpack2(uint32_t w, __nv_bfloat16) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+}
+__device__ __forceinline__ uint32_t pack2(float x, float y, __half) {
+  const __half2 h = __floats2half2_rn(x, y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pack2(float x, float y, __nv_bfloat16) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float2 turn2(float x, float y, float c, float s) { return make_float2(fmaf(x, c, -(y * s)), fmaf(y, c, x * s)); }
+
+// The V pairs of two chunks, turned in place.
 template <typename T, int V, bool INTERLEAVED>
-__global__ void __launch_bounds__(kRotThreads) rotary_kernel(const RotaryArgs a) {
-  extern __shared__ float s_cs[];  // [tokens][cos rot / 2, sin rot / 2]
-  using C = Chunk<T, V>;
-  const int half = a.rot / 2;
-  const int64_t t0 = (int64_t)blockIdx.x * a.tokens;
-  const int nt = (int)min((int64_t)a.tokens, a.n_tokens - t0);
-  const int heads = a.heads[0] + a.heads[1], per_token = heads * a.per_head;
-  // this block's share of the tokens' items
-  const int all = nt * per_token, share = (all + (int)gridDim.y - 1) / (int)gridDim.y;
-  const int i_end = min(all, ((int)blockIdx.y + 1) * share);
-
-  C lo[kRotBatch], hi[kRotBatch];
-  auto locate = [&](int i, int& tok, int& src, int& h, int& e) {
-    tok = i / per_token;
-    const int r = i - tok * per_token;
-    h = r / a.per_head;
-    e = r - h * a.per_head;
-    src = h >= a.heads[0] ? 1 : 0;
-    h -= src ? a.heads[0] : 0;
-  };
-  auto first_of = [&](int e) { return e >= a.turned ? a.rot + (e - a.turned) * V : INTERLEAVED ? 2 * V * e : V * e; };
-  const int step = INTERLEAVED ? V : half;  // from an item's first chunk to its second
-  auto load = [&](int i, C& x, C& y) {
-    int tok, src, h, e;
-    locate(i, tok, src, h, e);
-    const T* p = reinterpret_cast<const T*>(a.x[src]) + (t0 + tok) * a.x_token_stride[src] + (int64_t)h * a.x_head_stride[src] + first_of(e);
-    x = *reinterpret_cast<const C*>(p);
-    if (e < a.turned) y = *reinterpret_cast<const C*>(p + step);
-  };
-  auto turn = [&](int i, const C& x, const C& y) {
-    int tok, src, h, e;
-    locate(i, tok, src, h, e);
-    T* p = reinterpret_cast<T*>(a.y[src]) + (t0 + tok) * a.y_token_stride[src] + (int64_t)h * a.y_head_stride[src] + first_of(e);
-    if (e >= a.turned) {
-      *reinterpret_cast<C*>(p) = x;
-      return;
-    }
-    const float* c = s_cs + tok * a.rot + V * e;
-    const float* s = c + half;
-    C u, w;
+__device__ __forceinline__ void turn(Chunk<T, V>& x, Chunk<T, V>& y, const float (&c)[V], const float (&s)[V]) {
+  if constexpr (sizeof(T) == 4 && (V == 1 || !INTERLEAVED)) {
 #pragma unroll
     for (int k = 0; k < V; ++k) {
-      // pair k: elements k of the two chunks, or neighbours of the 2 V elements
-      const float p0 = INTERLEAVED ? to_float<T>(2 * k < V ? x.v[(2 * k) % V] : y.v[(2 * k) % V]) : to_float<T>(x.v[k]);
-      const float p1 = INTERLEAVED ? to_float<T>(2 * k + 1 < V ? x.v[(2 * k + 1) % V] : y.v[(2 * k + 1) % V]) : to_float<T>(y.v[k]);
-      const T q0 = from_float<T>(fmaf(p0, c[k], -(p1 * s[k]))), q1 = from_float<T>(fmaf(p1, c[k], p0 * s[k]));
-      if (!INTERLEAVED) {
-        u.v[k] = q0;
-        w.v[k] = q1;
-      } else {
-        (2 * k < V ? u : w).v[(2 * k) % V] = q0;
-        (2 * k + 1 < V ? u : w).v[(2 * k + 1) % V] = q1;
-      }
+      const float2 r = turn2(__uint_as_float(x.w[k]), __uint_as_float(y.w[k]), c[k], s[k]);
+      x.w[k] = __float_as_uint(r.x);
+      y.w[k] = __float_as_uint(r.y);
     }
-    *reinterpret_cast<C*>(p) = u;
-    *reinterpret_cast<C*>(p + step) = w;
-  };
-
-  int i = (int)blockIdx.y * share + (int)threadIdx.x;
+  } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
-  for (int b = 0; b < kRotBatch; ++b)
-    if (i + b * kRotThreads < i_end) load(i + b * kRotThreads, lo[b], hi[b]);
-  for (int k = threadIdx.x; k < nt * half; k += kRotThreads) {
-    const int tok = k / half, j = k - tok * half;
-    const int64_t pos = a.positions_64 ? reinterpret_cast<const int64_t*>(a.positions)[t0 + tok]
-                                       : (int64_t)reinterpret_cast<const int32_t*>(a.positions)[t0 + tok];
+    for (int k = 0; k < V; ++k) {
+      uint32_t* w = 2 * k < V ? x.w + 2 * k : y.w + (2 * k - V);
+      const float2 r = turn2(__uint_as_float(w[0]), __uint_as_float(w[1]), c[k], s[k]);
+      w[0] = __float_as_uint(r.x);
+      w[1] = __float_as_uint(r.y);
+    }
+  } else if constexpr (V == 1) {
+    const float2 r = turn2(unpack2(x.w[0], T()).x, unpack2(y.w[0], T()).x, c[0], s[0]);
+    x.w[0] = (uint16_t)pack2(r.x, 0.f, T());
+    y.w[0] = (uint16_t)pack2(r.y, 0.f, T());
+  } else if constexpr (INTERLEAVED) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      uint32_t& w = k < V / 2 ? x.w[k] : y.w[k - V / 2];
+      const float2 p = unpack2(w, T()), r = turn2(p.x, p.y, c[k], s[k]);
+      w = pack2(r.x, r.y, T());
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < V / 2; ++k) {
+      const float2 p = unpack2(x.w[k], T()), q = unpack2(y.w[k], T());
+      const float2 r0 = turn2(p.x, q.x, c[2 * k], s[2 * k]), r1 = turn2(p.y, q.y, c[2 * k + 1], s[2 * k + 1]);
+      x.w[k] = pack2(r0.x, r1.x, T());
+      y.w[k] = pack2(r0.y, r1.y, T());
+    }
+  }
+}
+
+// V elements of one type are moved at a time.  An item is the two chunks whose elements make V pairs (half layout: V i and
+// rot / 2 + V i; interleaved: 2 V i and the one behind it), or one chunk of the dimensions that do not turn.  A thread has one item's
+// place in some heads of a token, so what it needs of cosines and sines stays in its registers and nothing is divided on the way.
+// (With the items of a token dealt out flat, two divisions a chunk, 8 x 2048 tokens of 32 / 8 heads took 123 us, bound by issue.)
+template <typename T, int V, bool INTERLEAVED>
+__global__ void __launch_bounds__(kRotThreads, 3) rotary_kernel(const RotaryArgs a) {
+  extern __shared__ float s_cs[];  // [tokens][cos rot / 2, sin rot / 2]
+  using C = Chunk<T, V>;
+  const int half = a.rot / 2, tid = threadIdx.x;
+  const int64_t t0 = (int64_t)blockIdx.x * a.tokens;
+  const int nt = (int)min((int64_t)a.tokens, a.n_tokens - t0);
+  const int per_token = a.lanes * a.per_head, slot = tid / per_token, r = tid - slot * per_token;
+  const int lane = r / a.per_head, e = r - lane * a.per_head + (int)blockIdx.z * a.per_head;  // (items fastest: neighbours move neighbouring chunks)
+  const bool act = slot < a.pass && e < a.items, turned = e < a.turned;
+  const int at = !turned ? a.rot + (e - a.turned) * V : INTERLEAVED ? 2 * V * e : V * e;
+  const int step = INTERLEAVED ? V : half;  // from an item's first chunk to its second
+  const int heads = a.heads[0] + a.heads[1];
+  C lo[kRotBatch], hi[kRotBatch];
+  const T *xq, *xk;
+  T *yq, *yk;
+  auto token = [&](int t) {
+    xq = reinterpret_cast<const T*>(a.x[0]) + (t0 + t) * a.x_token_stride[0] + at;
+    xk = reinterpret_cast<const T*>(a.x[1]) + (t0 + t) * a.x_token_stride[1] + at;
+    yq = reinterpret_cast<T*>(a.y[0]) + (t0 + t) * a.y_token_stride[0] + at;
+    yk = reinterpret_cast<T*>(a.y[1]) + (t0 + t) * a.y_token_stride[1] + at;
+  };
+  auto load = [&](int h, C& x, C& y) {
+    const int k = h - a.heads[0];
+    const T* p = k < 0 ? xq + (int64_t)h * a.x_head_stride[0] : xk + (int64_t)k * a.x_head_stride[1];
+    x = *reinterpret_cast<const C*>(p);
+    if (turned) y = *reinterpret_cast<const C*>(p + step);
+  };
+  auto batch = [&](int h0) {
+#pragma unroll
+    for (int b = 0; b < kRotBatch; ++b)
+      if (h0 + b * a.lanes < heads) load(h0 + b * a.lanes, lo[b], hi[b]);
+  };
+  const int first = lane + (int)blockIdx.y * kRotBatch * a.lanes, stride = (int)gridDim.y * kRotBatch * a.lanes;
+  if (act && slot < nt && first < heads) {
+    token(slot);
+    batch(first);
+  }
+  // ---- the block's cosines and sines, while the first vectors are on their way -------------------------------
+  for (int k = tid; k < nt * half; k += kRotThreads) {
+    const int t = k / half, j = k - t * half;
     const double w = a.inv_freq_64 ? reinterpret_cast<const double*>(a.inv_freq)[j] : (double)reinterpret_cast<const float*>(a.inv_freq)[j];
+    const int64_t pos = a.positions_64 ? reinterpret_cast<const int64_t*>(a.positions)[t0 + t]
+                                       : (int64_t)reinterpret_cast<const int32_t*>(a.positions)[t0 + t];
     double turns = w * 0.15915494309189533577;  // 1 / (2 pi)
     turns -= floor(turns);
     const uint64_t frac = (uint64_t)(turns * 18446744073709551616.0) * (uint64_t)pos;
     float s, c;
     sincospif((float)(int32_t)(frac >> 32) * 0x1p-31f, &s, &c);
     if (!isfinite(w)) s = c = __int_as_float(0x7fffffff);
-    s_cs[tok * a.rot + j] = c * a.factor;
-    s_cs[tok * a.rot + half + j] = (a.inverse ? -s : s) * a.factor;
+    s_cs[t * a.rot + j] = c * a.factor;
+    s_cs[t * a.rot + half + j] = (a.inverse ? -s : s) * a.factor;
   }
   __syncthreads();
-  for (; i < i_end; i += kRotBatch * kRotThreads) {
+  if (!act) return;
+  for (int t = slot; t < nt; t += a.pass) {
+    float c[V], s[V];
+    if (turned) {
 #pragma unroll
-    for (int b = 0; b < kRotBatch; ++b)
-      if (i + b * kRotThreads < i_end) turn(i + b * kRotThreads, lo[b], hi[b]);
-    const int n = i + kRotBatch * kRotThreads;
+      for (int k = 0; k < V; ++k) {
+        c[k] = s_cs[t * a.rot + V * e + k];
+        s[k] = s_cs[t * a.rot + half + V * e + k];
+      }
+    }
+    for (int h0 = first; h0 < heads; h0 += stride) {
+      if (t != slot || h0 != first) {
+        if (h0 == first) token(t);
+        batch(h0);
+      }
 #pragma unroll
-    for (int b = 0; b < kRotBatch; ++b)
-      if (n + b * kRotThreads < i_end) load(n + b * kRotThreads, lo[b], hi[b]);
+      for (int b = 0; b < kRotBatch; ++b) {
+        const int h = h0 + b * a.lanes, hk = h - a.heads[0];
+        if (h >= heads) continue;
+        T* p = hk < 0 ? yq + (int64_t)h * a.y_head_stride[0] : yk + (int64_t)hk * a.y_head_stride[1];
+        if (turned) {
+          turn<T, V, INTERLEAVED>(lo[b], hi[b], c, s);
+          *reinterpret_cast<C*>(p + step) = hi[b];
+        }
+        *reinterpret_cast<C*>(p) = lo[b];
+      }
+    }
   }
 }
 
 template <typename T, int V, bool INTERLEAVED>
 int launch_rotary(RotaryArgs a, int head_dim, bool through, cudaStream_t st) {
   a.turned = a.rot / 2 / V;
-  a.per_head = a.turned + (through ? (head_dim - a.rot) / V : 0);
-  const int64_t per_token = (int64_t)(a.heads[0] + a.heads[1]) * a.per_head;
-  if (per_token > (1 << 24)) return TQ4_ERR_UNSUPPORTED;
-  // A batch of every thread's is a block's work, when there are blocks enough; few tokens: their heads are dealt out
-  int tokens = (int)(kRotBatch * kRotThreads / per_token);
-  const int64_t fill = 4 * (int64_t)sm_count();
-  if (tokens > a.n_tokens / fill) tokens = (int)(a.n_tokens / fill);
-  if (tokens > kRotMaxDim * 8 / a.rot) tokens = kRotMaxDim * 8 / a.rot;
-  if (tokens < 1) tokens = 1;
-  a.tokens = tokens;
-  const int64_t blocks = (a.n_tokens + tokens - 1) / tokens;
+  a.items = a.turned + (through ? (head_dim - a.rot) / V : 0);
+  a.per_head = a.items < kRotThreads ? a.items : kRotThreads;
+  const int groups = (a.items + a.per_head - 1) / a.per_head;
+  const int heads = a.heads[0] + a.heads[1], fit = kRotThreads / a.per_head;
+  // Many tokens: a batch of heads for every thread, so that its cosines serve them all, and two passes of tokens a block.  Few: as many
+  // threads a token as there are heads, and what a block cannot take dealt over several.
+  const bool many = a.n_tokens * heads * a.per_head >= (int64_t)4 * kRotThreads * kRotBatch * sm_count();
+  a.lanes = many ? (heads + kRotBatch - 1) / kRotBatch : heads;
+  if (a.lanes > fit) a.lanes = fit;
+  a.pass = fit / a.lanes;
+  a.tokens = many ? 2 * a.pass : a.pass;
+  while (a.tokens > 1 && a.tokens * a.rot > 8 * kRotMaxDim) --a.tokens;
+  if (a.pass > a.tokens) a.pass = a.tokens;
+  const int64_t blocks = (a.n_tokens + a.tokens - 1) / a.tokens;
   if (blocks > 0x7fffffff) return TQ4_ERR_UNSUPPORTED;
-  int64_t split = fill / 2 / blocks;
-  if (split > per_token / kRotThreads) split = per_token / kRotThreads;
-  if (split < 1) split = 1;
-  if (launch_kernel(rotary_kernel<T, V, INTERLEAVED>, dim3((unsigned)blocks, (unsigned)split), dim3(kRotThreads),
-                    (size_t)tokens * a.rot * sizeof(float), st, false, a) != cudaSuccess)
+  const int split = many ? 1 : (heads + kRotBatch * a.lanes - 1) / (kRotBatch * a.lanes);
+  if (split > 65535 || groups > 65535) return TQ4_ERR_UNSUPPORTED;
+  if (launch_kernel(rotary_kernel<T, V, INTERLEAVED>, dim3((unsigned)blocks, (unsigned)split, (unsigned)groups), dim3(kRotThreads),
+                    (size_t)a.tokens * a.rot * sizeof(float), st, false, a) != cudaSuccess)
     return TQ4_ERR_CUDA;
   TQ4_CHECK_LAUNCH();
   return TQ4_OK;

@@ -2,7 +2,9 @@
 //
 // Both move the H (D + 8) bytes of a token row that carry data, never its padding.  They are bound by HBM where there is much to
 // move and by two or three dependent round trips to memory (list, block table, rows) where there is little, so a launch covers
-// every layer, and a thread asks for several pieces of rows before it stores the first.
+// every layer.  Rows that start on 16 bytes and are a multiple of them go through shared memory by bulk copies, a row each, which
+// cost a lane two instructions a row and keep whole pages in flight; others (an odd number of heads) by 8- or 4-byte loads, several a
+// thread before the first is stored.
 #include "tq4_common.cuh"
 
 namespace tq4 {
@@ -11,10 +13,10 @@ namespace {
 constexpr int kMaxLayers = 128;   // caches a launch takes (their addresses travel with it)
 constexpr int kThreads = 256;
 constexpr int kBatch = 8;         // pieces a thread has in flight
-constexpr int kScanPairs = 1024;  // copies that every block compares its own with; above, a map of the pages is made first
+constexpr int kScanPairs = 256;   // copies that every block compares its own with; above, a map of the pages is made first
+constexpr int kStages = 4;        // sets of rows that a block of copies has under way
+constexpr uint32_t kStageBytes = 17408;  // ... of at most so many bytes, and a row a lane
 constexpr int kShortKeep = 64;    // kept rows of a sequence that one block sees to
-constexpr int kSegBytes = 32768;  // of the rows of a block otherwise
-constexpr int kMaxSegRows = 64;
 
 struct Caches {
   uint8_t* at[kMaxLayers];
@@ -40,6 +42,37 @@ __device__ __forceinline__ void report(int* flag, int bits) {
   if (flag) atomicOr(flag, bits);
 }
 
+__device__ __forceinline__ uint32_t smem_of(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void bulk_in(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void bulk_out(void* dst, uint32_t src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+// the lane's copies out of shared memory: all but the last `N` sets have been read from it / all have been written
+template <int N>
+__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+__device__ __forceinline__ void bar_init(uint32_t bar) { asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+// Bounded wait for copies of this warp's own.
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity) {
+  for (int it = 0; it < (1 << 22); ++it) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+    if (done) return true;
+  }
+  return false;
+}
+
 // ======================================================================================
 // Pages copied
 // ======================================================================================
@@ -49,6 +82,7 @@ struct CopyArgs {
   int pairs_64;
   int64_t n;
   int layers, per_block;  // caches; ... of a block
+  int rows;               // (bulk copies) of a stage
   const unsigned* claim;  // (many pairs) first pair with this destination, by page; ~0: none
   int* err_flag;
 };
@@ -64,28 +98,22 @@ __global__ void __launch_bounds__(kThreads) claim_kernel(const CopyArgs a, unsig
   if (src != dst && src >= 0 && src < a.g.num_blocks && dst >= 0 && dst < a.g.num_blocks) atomicMin(claim + dst, (unsigned)i);
 }
 
-template <int U>
-__global__ void __launch_bounds__(kThreads) copy_blocks_kernel(const __grid_constant__ Caches caches, const CopyArgs a) {
-  using T = typename Piece<U>::T;
-  const int groups = (a.layers + a.per_block - 1) / a.per_block;
-  const int64_t pair = blockIdx.x / groups;
-  const int layer0 = ((int)blockIdx.x % groups) * a.per_block, layer1 = min(a.layers, layer0 + a.per_block);
-  const int64_t src = index_at(a.pairs, a.pairs_64, 2 * pair), dst = index_at(a.pairs, a.pairs_64, 2 * pair + 1);
+// Whether pair (src, dst) is to be carried out; what is wrong with it is reported.  (All threads of the block.)
+__device__ __forceinline__ bool pair_counts(const CopyArgs& a, int64_t pair, int64_t src, int64_t dst) {
   if (a.claim) pdl_wait();
   const bool in_range = src >= 0 && src < a.g.num_blocks && dst >= 0 && dst < a.g.num_blocks;
   if (!in_range) {
     if (threadIdx.x == 0) report(a.err_flag, TQ4_DEV_BAD_BLOCK);
-    return;
+    return false;
   }
-  if (src == dst) return;
-  // ---- is this pair to be carried out? -----------------------------------------------------------------
+  if (src == dst) return false;
   int skip = 0, clash = 0;
   if (a.claim) {
     const unsigned first = a.claim[dst];
     skip = first != (unsigned)pair;
     clash = (skip && index_at(a.pairs, a.pairs_64, 2 * (int64_t)first) != src) || a.claim[src] != ~0u;
   } else {
-    for (int i = threadIdx.x; i < (int)a.n; i += kThreads) {
+    for (int i = threadIdx.x; i < (int)a.n; i += blockDim.x) {
       const int64_t s = index_at(a.pairs, a.pairs_64, 2 * i), d = index_at(a.pairs, a.pairs_64, 2 * i + 1);
       if (s == d || s < 0 || s >= a.g.num_blocks) continue;
       if (d == dst && i < (int)pair) {
@@ -98,7 +126,17 @@ __global__ void __launch_bounds__(kThreads) copy_blocks_kernel(const __grid_cons
     clash = __syncthreads_or(clash);
   }
   if (clash && threadIdx.x == 0) report(a.err_flag, TQ4_DEV_PAGE_CONFLICT);
-  if (skip || clash) return;
+  return !skip && !clash;
+}
+
+template <int U>
+__global__ void __launch_bounds__(kThreads) copy_blocks_kernel(const __grid_constant__ Caches caches, const CopyArgs a) {
+  using T = typename Piece<U>::T;
+  const int groups = (a.layers + a.per_block - 1) / a.per_block;
+  const int64_t pair = blockIdx.x / groups;
+  const int layer0 = ((int)blockIdx.x % groups) * a.per_block, layer1 = min(a.layers, layer0 + a.per_block);
+  const int64_t src = index_at(a.pairs, a.pairs_64, 2 * pair), dst = index_at(a.pairs, a.pairs_64, 2 * pair + 1);
+  if (!pair_counts(a, pair, src, dst)) return;
   // ---- the page, layer by layer ---------------------------------------------------------------------------
   const int page = a.g.block_size * a.g.row_units, all = page * (layer1 - layer0);
   for (int i0 = threadIdx.x; i0 < all; i0 += kBatch * kThreads) {
@@ -118,6 +156,51 @@ __global__ void __launch_bounds__(kThreads) copy_blocks_kernel(const __grid_cons
       if (i < all) *reinterpret_cast<T*>(caches.at[layer0 + i / page] + dst * a.g.block_stride + at[b]) = x[b];
     }
   }
+}
+
+// The same by bulk copies: one warp, a lane a row of the set of rows that a stage holds.  A lane stores what it loaded itself, so it
+// may ask for its next row as soon as its own copy out of that place has read it.
+__global__ void __launch_bounds__(32) copy_blocks_bulk_kernel(const __grid_constant__ Caches caches, const CopyArgs a) {
+  extern __shared__ __align__(128) unsigned char s_rows[];
+  __shared__ __align__(8) uint64_t s_bar[kStages];
+  const int lane = threadIdx.x;
+  const int groups = (a.layers + a.per_block - 1) / a.per_block;
+  const int64_t pair = blockIdx.x / groups;
+  const int layer0 = ((int)blockIdx.x % groups) * a.per_block, layers = min(a.layers - layer0, a.per_block);
+  const int64_t src = index_at(a.pairs, a.pairs_64, 2 * pair), dst = index_at(a.pairs, a.pairs_64, 2 * pair + 1);
+  const uint32_t bytes = (uint32_t)a.g.row_units * 16, slot = smem_of(s_rows) + lane * bytes;
+  if (lane < kStages) bar_init(smem_of(&s_bar[lane]));
+  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  __syncwarp();
+  if (!pair_counts(a, pair, src, dst)) return;
+  const int sets = (a.g.block_size + a.rows - 1) / a.rows, all = sets * layers;  // of a page; of the block
+  const uint32_t stage = a.rows * bytes;
+  auto rows_of = [&](int i) { return min(a.rows, a.g.block_size - (i % sets) * a.rows); };
+  auto at = [&](int i, int64_t page) {
+    return caches.at[layer0 + i / sets] + page * a.g.block_stride + (int64_t)((i % sets) * a.rows + lane) * a.g.token_stride;
+  };
+  auto ask = [&](int i) {
+    const int n = rows_of(i);
+    const uint32_t bar = smem_of(&s_bar[i % kStages]);
+    if (lane == 0) bar_expect(bar, n * bytes);
+    __syncwarp();
+    if (lane < n) bulk_in(slot + (i % kStages) * stage, at(i, src), bytes, bar);
+  };
+  for (int i = 0; i < min(kStages, all); ++i) ask(i);
+  for (int i = 0; i < all; ++i) {
+    if (!bar_wait(smem_of(&s_bar[i % kStages]), (i / kStages) & 1)) {
+      report(a.err_flag, TQ4_DEV_TIMEOUT);
+      for (int k = i + 1; k < min(i + kStages, all); ++k) bar_wait(smem_of(&s_bar[k % kStages]), (k / kStages) & 1);  // (copies under way)
+      break;
+    }
+    if (lane < rows_of(i)) bulk_out(at(i, dst), slot + (i % kStages) * stage, bytes);
+    bulk_commit();
+    if (i > 0 && i - 1 + kStages < all) {
+      bulk_wait_read<1>();
+      ask(i - 1 + kStages);
+    }
+  }
+  bulk_wait_all();
 }
 
 // ======================================================================================
@@ -257,8 +340,8 @@ __device__ __forceinline__ int lower_bound_warp(const int32_t* keep, int n, int 
 template <int U>
 __global__ void __launch_bounds__(kThreads) compact_long_kernel(const __grid_constant__ Caches caches, const CompactArgs a) {
   using T = typename Piece<U>::T;
-  extern __shared__ __align__(16) unsigned char s_rows[];
-  __shared__ int64_t s_src[kMaxSegRows], s_dst[kMaxSegRows];
+  extern __shared__ __align__(128) unsigned char s_rows[];
+  __shared__ int64_t s_src[32], s_dst[32];
   __shared__ int s_ticket, s_range[2], s_stuck;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   pdl_wait();
@@ -294,10 +377,7 @@ __global__ void __launch_bounds__(kThreads) compact_long_kernel(const __grid_con
     const int row = i / a.g.row_units;
     if (s_src[row] < 0) continue;
     const uint8_t* from = cache + s_src[row] + (i - row * a.g.row_units) * U;
-    if constexpr (U == 16)
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(base + i * U), "l"(from) : "memory");
-    else
-      asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(base + i * U), "l"(from), "n"(U) : "memory");
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(base + i * U), "l"(from), "n"(U) : "memory");
   }
   // rows k < j0 that come from the places of this block's rows
   if (warp < 2) {
@@ -314,7 +394,7 @@ __global__ void __launch_bounds__(kThreads) compact_long_kernel(const __grid_con
   if (s_range[0] < s_range[1]) {
     for (int s = s_range[0] / a.seg_rows + tid; s <= (s_range[1] - 1) / a.seg_rows; s += kThreads) {
       int there = 0;
-      for (int it = 0; it < (1 << 22) && !there; ++it)
+      for (int it = 0; it < (1 << 20) && !there; ++it)
         asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(there) : "l"(loaded + s) : "memory");
       if (!there) s_stuck = 1;
     }
@@ -331,6 +411,67 @@ __global__ void __launch_bounds__(kThreads) compact_long_kernel(const __grid_con
   }
 }
 
+// The same by bulk copies: one warp, a row a lane.
+__global__ void __launch_bounds__(32) compact_long_bulk_kernel(const __grid_constant__ Caches caches, const CompactArgs a) {
+  extern __shared__ __align__(128) unsigned char s_rows[];
+  __shared__ __align__(8) uint64_t s_bar;
+  const int lane = threadIdx.x;
+  const uint32_t bar = smem_of(&s_bar), bytes = (uint32_t)a.g.row_units * 16, slot = smem_of(s_rows) + lane * bytes;
+  if (lane == 0) bar_init(bar);
+  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  pdl_wait();
+  int ticket = 0;
+  if (lane == 0) ticket = atomicAdd(a.ticket, 1);
+  ticket = __shfl_sync(0xffffffffu, ticket, 0);
+  const int per_seg = a.layers * a.seqs, seg = ticket / per_seg, rest = ticket - seg * per_seg;
+  const int seq = rest / a.layers, layer = rest - seq * a.layers;
+  const int j0 = seg * a.seg_rows, rows = min(a.seg_rows, a.valid[seq] - j0);
+  if (rows <= 0) return;
+  const int32_t* keep = a.keep + seq * a.keep_stride;
+  const int64_t first = a.first[seq];
+  int64_t src = -1, dst = -1;
+  if (lane < rows) {
+    const int k = keep[j0 + lane];
+    const int32_t* table = a.table + seq * a.table_stride;
+    if (k != j0 + lane) {
+      src = row_at(a, table, first + k);
+      dst = row_at(a, table, first + j0 + lane);
+    }
+  }
+  const bool moves = src >= 0 && dst >= 0;
+  const unsigned movers = __ballot_sync(0xffffffffu, moves);
+  if (lane == 0) bar_expect(bar, __popc(movers) * bytes);
+  __syncwarp();
+  uint8_t* cache = caches.at[layer];
+  if (moves) bulk_in(slot, cache + src, bytes, bar);
+  // rows k < j0 that come from the places of this block's rows
+  const int k0 = lower_bound_warp(keep, j0, j0, lane), k1 = lower_bound_warp(keep, j0, j0 + rows, lane);
+  bool ok = bar_wait(bar, 0);
+  int* loaded = a.loaded + ((int64_t)layer * a.seqs + seq) * a.segments;
+  __syncwarp();
+  if (lane == 0) {
+    __threadfence();
+    asm volatile("st.release.gpu.global.s32 [%0], 1;" ::"l"(loaded + seg) : "memory");
+  }
+  if (k0 < k1) {
+    for (int s = k0 / a.seg_rows + lane; s <= (k1 - 1) / a.seg_rows; s += 32) {
+      int there = 0;
+      for (int it = 0; it < (1 << 20) && !there; ++it)
+        asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(there) : "l"(loaded + s) : "memory");
+      ok = ok && there;
+    }
+    __threadfence();
+  }
+  if (!__all_sync(0xffffffffu, ok)) {
+    if (lane == 0) report(a.err_flag, TQ4_DEV_TIMEOUT);
+    return;
+  }
+  asm volatile("fence.proxy.async;" ::: "memory");  // the marks were read like any memory, the copies are not
+  if (moves) bulk_out(cache + dst, slot, bytes);
+  bulk_commit();
+  bulk_wait_all();
+}
+
 // Largest piece that the caches' addresses and strides, and the bytes of a row, are multiples of.
 int piece_of(const Caches& c, int layers, int64_t block_stride, int64_t token_stride, int row_bytes) {
   uintptr_t all = (uintptr_t)block_stride | (uintptr_t)token_stride | (uintptr_t)row_bytes | 16;
@@ -338,9 +479,10 @@ int piece_of(const Caches& c, int layers, int64_t block_stride, int64_t token_st
   return all % 16 == 0 ? 16 : all % 8 == 0 ? 8 : 4;
 }
 
-int seg_rows_of(int row_bytes) {
-  const int n = kSegBytes / row_bytes;
-  return n < 1 ? 1 : n > kMaxSegRows ? kMaxSegRows : n;
+// rows of a bulk copy's stage, or of a segment of a long list
+int stage_rows(int row_bytes) {
+  const int n = (int)kStageBytes / row_bytes;
+  return n < 1 ? 1 : n > 32 ? 32 : n;
 }
 
 struct CompactSpace {
@@ -349,7 +491,7 @@ struct CompactSpace {
 };
 CompactSpace compact_space(int layers, int seqs, int keep_width, int row_bytes) {
   CompactSpace s{};
-  s.segments = (keep_width + seg_rows_of(row_bytes) - 1) / seg_rows_of(row_bytes);
+  s.segments = (keep_width + stage_rows(row_bytes) - 1) / stage_rows(row_bytes);
   s.valid = 16;
   s.loaded = s.valid + ((size_t)seqs * 4 + 15) / 16 * 16;
   s.bytes = s.loaded + (size_t)(layers < kMaxLayers ? layers : kMaxLayers) * seqs * s.segments * 4;
@@ -368,8 +510,27 @@ int check_caches(uint8_t* const* caches, int layers, int64_t num_blocks, int blo
   return TQ4_OK;
 }
 
+int launch_copy_bulk(const Caches& c, CopyArgs a, cudaStream_t st) {
+  const int row_bytes = a.g.row_units * 16;
+  a.rows = stage_rows(row_bytes);
+  if (a.rows > a.g.block_size) a.rows = a.g.block_size;
+  const size_t smem = (size_t)kStages * a.rows * row_bytes;
+  if (!ensure_dynamic_smem<copy_blocks_bulk_kernel>((int)smem, true)) return TQ4_ERR_CUDA;
+  // Layers of a block: enough blocks to fill the GPU at few pages, and as few looks at the list as there can be at many
+  const int64_t fill = 3 * (int64_t)sm_count();
+  const int64_t groups = fill / a.n < 1 ? 1 : fill / a.n < a.layers ? fill / a.n : a.layers;
+  a.per_block = (int)((a.layers + groups - 1) / groups);
+  const int64_t blocks = a.n * ((a.layers + a.per_block - 1) / a.per_block);
+  if (blocks > 0x7fffffff || (int64_t)a.per_block * a.g.block_size > 0x3fffffff) return TQ4_ERR_UNSUPPORTED;
+  if (launch_kernel(copy_blocks_bulk_kernel, dim3((unsigned)blocks), dim3(32), smem, st, a.claim != nullptr, c, a) != cudaSuccess) return TQ4_ERR_CUDA;
+  TQ4_CHECK_LAUNCH();
+  return TQ4_OK;
+}
+
 template <int U>
 int launch_copy(const Caches& c, CopyArgs a, cudaStream_t st) {
+  if constexpr (U == 16)
+    if (kStages * a.g.row_units * 16 <= 200 * 1024) return launch_copy_bulk(c, a, st);
   // A block moves about 32 KB: enough blocks to fill the GPU at few pages, and no more than one look at the list for each
   const int page = a.g.block_size * a.g.row_units;
   a.per_block = (kBatch * kThreads + page - 1) / page;
@@ -398,13 +559,21 @@ int launch_compact(const Caches& c, CompactArgs a, int row_bytes, cudaStream_t s
   const int64_t grid = (int64_t)a.seqs * a.layers * a.segments;
   const size_t smem = (size_t)a.seg_rows * row_bytes;
   if (grid > 0x7fffffff || smem > 200 * 1024) return TQ4_ERR_UNSUPPORTED;
-  if (!ensure_dynamic_smem<compact_long_kernel<U>>((int)smem, true)) return TQ4_ERR_CUDA;
+  constexpr bool bulk = U == 16;
+  if constexpr (bulk) {
+    if (!ensure_dynamic_smem<compact_long_bulk_kernel>((int)smem, true)) return TQ4_ERR_CUDA;
+  } else {
+    if (!ensure_dynamic_smem<compact_long_kernel<U>>((int)smem, true)) return TQ4_ERR_CUDA;
+  }
   const int64_t marks = (grid + 1023) / 1024, most = sm_count();
   const int64_t blocks = marks > a.seqs ? marks : a.seqs;
   if (launch_kernel(compact_check_kernel, dim3((unsigned)(blocks < most ? blocks : most)), dim3(1024), 0, st, false, a) != cudaSuccess)
     return TQ4_ERR_CUDA;
   TQ4_CHECK_LAUNCH();
-  if (launch_kernel(compact_long_kernel<U>, dim3((unsigned)grid), dim3(kThreads), smem, st, true, c, a) != cudaSuccess) return TQ4_ERR_CUDA;
+  cudaError_t e;
+  if constexpr (bulk) e = launch_kernel(compact_long_bulk_kernel, dim3((unsigned)grid), dim3(32), smem, st, true, c, a);
+  else e = launch_kernel(compact_long_kernel<U>, dim3((unsigned)grid), dim3(kThreads), smem, st, true, c, a);
+  if (e != cudaSuccess) return TQ4_ERR_CUDA;
   TQ4_CHECK_LAUNCH();
   return TQ4_OK;
 }
@@ -494,7 +663,7 @@ extern "C" int tq4_compact_rows(uint8_t* const* caches, int num_caches, int64_t 
     const CompactSpace s = compact_space(num_caches, num_seqs, keep_width, row_bytes);
     unsigned char* w = reinterpret_cast<unsigned char*>(workspace);
     a.segments = s.segments;
-    a.seg_rows = seg_rows_of(row_bytes);
+    a.seg_rows = stage_rows(row_bytes);
     a.ticket = reinterpret_cast<int*>(w + s.ticket);
     a.valid = reinterpret_cast<int*>(w + s.valid);
     a.loaded = reinterpret_cast<int*>(w + s.loaded);
