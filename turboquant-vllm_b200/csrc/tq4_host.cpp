@@ -703,7 +703,7 @@ PyObject* tree_mask(PyObject*, PyObject* const* p, Py_ssize_t n) {
     TQ4_ASSERT(parents.scalar_type() == at::kInt && parents.dim() == 1 && parents.is_contiguous(), "parents must be contiguous int32 [rows]");
     TQ4_ASSERT(qsl.scalar_type() == at::kInt && qsl.dim() == 1 && qsl.is_contiguous() && qsl.numel() > 0,
                "query_start_loc must be contiguous int32 [sequences + 1]");
-    TQ4_ASSERT(nodes > 0 && nodes <= (1 << 20), "max_nodes must be between 1 and 2^20");
+    TQ4_ASSERT(nodes > 0 && nodes <= (1 << 19), "max_nodes must be between 1 and 2^19");
     const int64_t rows = parents.numel(), words = (nodes + 31) / 32;
     Launch launch(dev);
     at::Tensor mask = at::empty({rows, words}, parents.options().requires_grad(false));

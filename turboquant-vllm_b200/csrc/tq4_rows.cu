@@ -217,6 +217,7 @@ struct CompactArgs {
   const int32_t* kept;       // [seqs]
   int32_t* lens_out;         // (optional) [seqs] first + kept
   int seqs, layers, per_block;
+  int rows;                  // (short lists, bulk copies) of a set
   // long lists
   int segments, seg_rows;    // segments of a sequence, rows of a segment
   int* ticket;
@@ -296,6 +297,59 @@ __global__ void __launch_bounds__(kThreads) compact_short_kernel(const __grid_co
     }
     __syncthreads();
   }
+}
+
+// The same by bulk copies: one warp, a lane a row of a layer, layer by layer and in ascending order; a set of them is loaded before the
+// first of it is stored.  (Accepted drafts of 64 trees of 16 in 32 layers: 9.5 us by loads of 16 bytes, most of it for dividing
+// them among the threads, 5.0 us so.)
+__global__ void __launch_bounds__(32) compact_short_bulk_kernel(const __grid_constant__ Caches caches, const CompactArgs a) {
+  extern __shared__ __align__(128) unsigned char s_rows[];
+  __shared__ __align__(8) uint64_t s_bar;
+  const int lane = threadIdx.x;
+  const uint32_t bar = smem_of(&s_bar), bytes = (uint32_t)a.g.row_units * 16, slot = smem_of(s_rows) + lane * bytes;
+  const int groups = (a.layers + a.per_block - 1) / a.per_block;
+  const int seq = (int)blockIdx.x / groups, layer0 = ((int)blockIdx.x % groups) * a.per_block;
+  const int layers = min(a.layers - layer0, a.per_block);
+  const int n = kept_of(a, seq);
+  const int32_t* keep = a.keep + seq * a.keep_stride;
+  const int32_t* table = a.table + seq * a.table_stride;
+  const int64_t first = a.first[seq];
+  if (lane == 0) {
+    bar_init(bar);
+    if (layer0 == 0 && a.lens_out) a.lens_out[seq] = a.first[seq] + a.kept[seq];
+  }
+  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  int bad = n < 0;
+  for (int j = lane; j < n; j += 32) bad |= keep[j] < 0 || (j > 0 && keep[j - 1] >= keep[j]);
+  if (__any_sync(0xffffffffu, bad)) {  // a list out of order: reported, the sequence is left as it is
+    if (lane == 0) report(a.err_flag, TQ4_DEV_KEEP_ORDER);
+    return;
+  }
+  const int all = n * layers;
+  for (int i0 = 0, phase = 0; i0 < all; i0 += a.rows, phase ^= 1) {
+    const int i = i0 + lane, layer = i / n, row = i - layer * n;
+    int64_t src = -1, dst = -1;
+    if (lane < a.rows && i < all && keep[row] != row) {  // (rows that stay where they are are not touched)
+      src = row_at(a, table, first + keep[row]);
+      dst = row_at(a, table, first + row);
+    }
+    const bool moves = src >= 0 && dst >= 0;
+    const unsigned movers = __ballot_sync(0xffffffffu, moves);
+    if (lane == 0) bar_expect(bar, __popc(movers) * bytes);
+    __syncwarp();
+    if (moves) {
+      bulk_wait_read<0>();  // (the lane's row before is out of its place)
+      bulk_in(slot, caches.at[layer0 + layer] + src, bytes, bar);
+    }
+    if (!bar_wait(bar, phase)) {
+      report(a.err_flag, TQ4_DEV_TIMEOUT);
+      break;
+    }
+    __syncwarp();
+    if (moves) bulk_out(caches.at[layer0 + layer] + dst, slot, bytes);
+    bulk_commit();
+  }
+  bulk_wait_all();
 }
 
 // Long lists, first kernel: is each in order, and the marks of the second one to zero.
@@ -411,7 +465,9 @@ __global__ void __launch_bounds__(kThreads) compact_long_kernel(const __grid_con
   }
 }
 
-// The same by bulk copies: one warp, a row a lane.
+// The same by bulk copies: one warp, a row a lane.  One segment in one layer a block, with a dozen blocks an SM: with several layers
+// behind one another the mark's release waits for the copies out of the layer before (half of four contexts of 16384 in 8 layers:
+// 129 us with up to four layers a block, 112 so).
 __global__ void __launch_bounds__(32) compact_long_bulk_kernel(const __grid_constant__ Caches caches, const CompactArgs a) {
   extern __shared__ __align__(128) unsigned char s_rows[];
   __shared__ __align__(8) uint64_t s_bar;
@@ -419,6 +475,7 @@ __global__ void __launch_bounds__(32) compact_long_bulk_kernel(const __grid_cons
   const uint32_t bar = smem_of(&s_bar), bytes = (uint32_t)a.g.row_units * 16, slot = smem_of(s_rows) + lane * bytes;
   if (lane == 0) bar_init(bar);
   asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  __syncwarp();
   pdl_wait();
   int ticket = 0;
   if (lane == 0) ticket = atomicAdd(a.ticket, 1);
@@ -440,33 +497,28 @@ __global__ void __launch_bounds__(32) compact_long_bulk_kernel(const __grid_cons
   }
   const bool moves = src >= 0 && dst >= 0;
   const unsigned movers = __ballot_sync(0xffffffffu, moves);
+  uint8_t* cache = caches.at[layer];
   if (lane == 0) bar_expect(bar, __popc(movers) * bytes);
   __syncwarp();
-  uint8_t* cache = caches.at[layer];
   if (moves) bulk_in(slot, cache + src, bytes, bar);
-  // rows k < j0 that come from the places of this block's rows
+  // rows k < j0 that come from the places of this block's rows, and the segments that have them
   const int k0 = lower_bound_warp(keep, j0, j0, lane), k1 = lower_bound_warp(keep, j0, j0 + rows, lane);
   bool ok = bar_wait(bar, 0);
   int* loaded = a.loaded + ((int64_t)layer * a.seqs + seq) * a.segments;
   __syncwarp();
-  if (lane == 0) {
-    __threadfence();
-    asm volatile("st.release.gpu.global.s32 [%0], 1;" ::"l"(loaded + seg) : "memory");
-  }
-  if (k0 < k1) {
+  if (lane == 0) asm volatile("st.release.gpu.global.s32 [%0], 1;" ::"l"(loaded + seg) : "memory");
+  if (k0 < k1)
     for (int s = k0 / a.seg_rows + lane; s <= (k1 - 1) / a.seg_rows; s += 32) {
       int there = 0;
       for (int it = 0; it < (1 << 20) && !there; ++it)
         asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(there) : "l"(loaded + s) : "memory");
       ok = ok && there;
     }
-    __threadfence();
-  }
   if (!__all_sync(0xffffffffu, ok)) {
     if (lane == 0) report(a.err_flag, TQ4_DEV_TIMEOUT);
     return;
   }
-  asm volatile("fence.proxy.async;" ::: "memory");  // the marks were read like any memory, the copies are not
+  asm volatile("fence.proxy.async.global;" ::: "memory");  // the marks were read like any memory, the copies are not
   if (moves) bulk_out(cache + dst, slot, bytes);
   bulk_commit();
   bulk_wait_all();
@@ -480,8 +532,8 @@ int piece_of(const Caches& c, int layers, int64_t block_stride, int64_t token_st
 }
 
 // rows of a bulk copy's stage, or of a segment of a long list
-int stage_rows(int row_bytes) {
-  const int n = (int)kStageBytes / row_bytes;
+int stage_rows(int row_bytes, uint32_t stage = kStageBytes) {
+  const int n = (int)stage / row_bytes;
   return n < 1 ? 1 : n > 32 ? 32 : n;
 }
 
@@ -546,6 +598,19 @@ int launch_copy(const Caches& c, CopyArgs a, cudaStream_t st) {
 template <int U>
 int launch_compact(const Caches& c, CompactArgs a, int row_bytes, cudaStream_t st) {
   if (a.keep_width <= kShortKeep) {
+    if constexpr (U == 16) {
+      a.rows = stage_rows(row_bytes, 2 * kStageBytes);
+      const size_t smem = (size_t)a.rows * row_bytes;
+      a.per_block = a.keep_width < a.rows ? a.rows / (a.keep_width > 0 ? a.keep_width : 1) : 1;  // as many layers as make a set
+      if (a.per_block > a.layers) a.per_block = a.layers;
+      const int64_t grid = (int64_t)a.seqs * ((a.layers + a.per_block - 1) / a.per_block);
+      if (grid <= 0x7fffffff && smem <= 200 * 1024) {
+        if (!ensure_dynamic_smem<compact_short_bulk_kernel>((int)smem, true)) return TQ4_ERR_CUDA;
+        if (launch_kernel(compact_short_bulk_kernel, dim3((unsigned)grid), dim3(32), smem, st, false, c, a) != cudaSuccess) return TQ4_ERR_CUDA;
+        TQ4_CHECK_LAUNCH();
+        return TQ4_OK;
+      }
+    }
     // (a few rows a sequence: as many layers a block as make a batch of every thread's)
     a.per_block = kBatch * kThreads / (4 * a.g.row_units);
     if (a.per_block < 1) a.per_block = 1;
@@ -556,23 +621,22 @@ int launch_compact(const Caches& c, CompactArgs a, int row_bytes, cudaStream_t s
     TQ4_CHECK_LAUNCH();
     return TQ4_OK;
   }
-  const int64_t grid = (int64_t)a.seqs * a.layers * a.segments;
-  const size_t smem = (size_t)a.seg_rows * row_bytes;
-  if (grid > 0x7fffffff || smem > 200 * 1024) return TQ4_ERR_UNSUPPORTED;
+  const int64_t marks = (int64_t)a.seqs * a.layers * a.segments;
   constexpr bool bulk = U == 16;
+  const size_t smem = (size_t)a.seg_rows * row_bytes;
+  if (marks > 0x7fffffff || smem > 200 * 1024) return TQ4_ERR_UNSUPPORTED;
   if constexpr (bulk) {
     if (!ensure_dynamic_smem<compact_long_bulk_kernel>((int)smem, true)) return TQ4_ERR_CUDA;
   } else {
     if (!ensure_dynamic_smem<compact_long_kernel<U>>((int)smem, true)) return TQ4_ERR_CUDA;
   }
-  const int64_t marks = (grid + 1023) / 1024, most = sm_count();
-  const int64_t blocks = marks > a.seqs ? marks : a.seqs;
-  if (launch_kernel(compact_check_kernel, dim3((unsigned)(blocks < most ? blocks : most)), dim3(1024), 0, st, false, a) != cudaSuccess)
+  const int64_t want = (marks + 1023) / 1024 > a.seqs ? (marks + 1023) / 1024 : a.seqs, most = sm_count();
+  if (launch_kernel(compact_check_kernel, dim3((unsigned)(want < most ? want : most)), dim3(1024), 0, st, false, a) != cudaSuccess)
     return TQ4_ERR_CUDA;
   TQ4_CHECK_LAUNCH();
   cudaError_t e;
-  if constexpr (bulk) e = launch_kernel(compact_long_bulk_kernel, dim3((unsigned)grid), dim3(32), smem, st, true, c, a);
-  else e = launch_kernel(compact_long_kernel<U>, dim3((unsigned)grid), dim3(kThreads), smem, st, true, c, a);
+  if constexpr (bulk) e = launch_kernel(compact_long_bulk_kernel, dim3((unsigned)marks), dim3(32), smem, st, true, c, a);
+  else e = launch_kernel(compact_long_kernel<U>, dim3((unsigned)marks), dim3(kThreads), smem, st, true, c, a);
   if (e != cudaSuccess) return TQ4_ERR_CUDA;
   TQ4_CHECK_LAUNCH();
   return TQ4_OK;

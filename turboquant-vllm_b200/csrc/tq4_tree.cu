@@ -4,7 +4,8 @@
 namespace tq4 {
 namespace {
 
-constexpr int kMaskThreads = 256;
+constexpr int kMaskThreads = 128;
+constexpr int kMaskBytes = 96 * 1024;  // words of a block's rows
 constexpr int kMaskNodes = 2048;  // drafts of a sequence whose parents a block keeps in shared memory
 
 struct MaskArgs {
@@ -12,56 +13,58 @@ struct MaskArgs {
   const int32_t* starts;  // [seqs + 1]
   int64_t rows;
   int seqs, words;
+  int block_rows;         // rows of a block
   int32_t* mask;   // [rows][words]
   int32_t* depth;  // [rows]
   int* err_flag;
 };
 
-// Row j of a sequence: bits of j, its parent, the parent's parent, ...  A thread makes one word of a row: it walks up the whole
-// branch (parents in shared memory) and keeps the bits of its word, so a row's words are made side by side and stored once.
-// Bound by the walk's latency, about 30 cycles a step.
-// blockIdx.x: sequence (the one behind the last stands for rows of no sequence), blockIdx.y: share of its words
+// Row j of a sequence: bits of j, its parent, the parent's parent, ...  A thread walks up from one row, with the parents and the rows'
+// words in shared memory; a block then stores its rows' words side by side.  Bound by the walk, some 40 cycles a step.  (A thread for each
+// word of a row walked every branch once a word: 64 trees of 200 to 512 drafts 10.3 us, 7.2 us so.)
+// blockIdx.x: sequence (the one behind the last stands for rows of no sequence), blockIdx.y: share of its rows
 __global__ void __launch_bounds__(kMaskThreads) tree_mask_kernel(const MaskArgs a) {
+  extern __shared__ unsigned s_bits[];  // [rows of a block][pitch]
   __shared__ int s_parent[kMaskNodes];
-  const int seq = blockIdx.x;
-  const int64_t rows = a.rows;
-  int64_t r0, r1;
-  if (seq < a.seqs) {
-    r0 = min(max((int64_t)a.starts[seq], (int64_t)0), rows);
-    r1 = min(max((int64_t)a.starts[seq + 1], r0), rows);
-  } else {
-    r0 = min(max((int64_t)a.starts[a.seqs], (int64_t)0), rows);
-    r1 = rows;
-  }
-  const int64_t n = r1 - r0, items = n * a.words;
+  const int seq = blockIdx.x, tid = threadIdx.x;
+  int64_t r0 = min(max((int64_t)a.starts[seq], (int64_t)0), a.rows), r1 = a.rows;
+  if (seq < a.seqs) r1 = min(max((int64_t)a.starts[seq + 1], r0), a.rows);
+  const int n = (int)(r1 - r0), words = a.words, pitch = words | 1;  // (odd: rows lie in different banks)
   const bool held = n <= kMaskNodes;
-  if (seq < a.seqs && held) {
-    for (int i = threadIdx.x; i < (int)n; i += kMaskThreads) s_parent[i] = a.parents[r0 + i];
-    __syncthreads();
-  }
   const int32_t* parents = a.parents + r0;
-  for (int64_t i = (int64_t)blockIdx.y * kMaskThreads + threadIdx.x; i < items; i += (int64_t)gridDim.y * kMaskThreads) {
-    const int64_t j = i / a.words;
-    const int w = (int)(i - j * a.words);
-    unsigned bits = 0;
-    int depth = -1;
-    if (seq < a.seqs) {
-      // (a parent is an earlier draft: the walk goes down in j and ends)
-      int64_t k = j;
-      while (true) {
-        if ((k >> 5) == w) bits |= 1u << (k & 31);
-        ++depth;
-        const int p = held ? s_parent[k] : parents[k];
-        if (p < 0 || p >= k) {  // the first of its branch; what is no earlier draft is reported and ends the walk
-          if ((p < -1 || p >= k) && a.err_flag) atomicOr(a.err_flag, TQ4_DEV_BAD_TREE);
-          break;
+  if (seq < a.seqs && held && (int)blockIdx.y * a.block_rows < n)
+    for (int i = tid; i < n; i += kMaskThreads) s_parent[i] = parents[i];
+  for (int b0 = (int)blockIdx.y * a.block_rows; b0 < n; b0 += (int)gridDim.y * a.block_rows) {
+    const int rows = min(a.block_rows, n - b0);
+    for (int i = tid; i < rows * pitch; i += kMaskThreads) s_bits[i] = 0u;
+    __syncthreads();
+    for (int i = tid; i < rows; i += kMaskThreads) {
+      const int j = b0 + i;
+      int depth = -1;
+      if (seq < a.seqs) {
+        unsigned* mine = s_bits + i * pitch;
+        int k = j;
+        while (true) {  // (a parent is an earlier draft: the walk goes down in k and ends)
+          if ((k >> 5) < words) mine[k >> 5] |= 1u << (k & 31);
+          ++depth;
+          const int p = held ? s_parent[k] : parents[k];
+          if (p < 0 || p >= k) {  // the first of its branch; what is no earlier draft is reported and ends the walk
+            if ((p < -1 || p >= k) && a.err_flag) atomicOr(a.err_flag, TQ4_DEV_BAD_TREE);
+            break;
+          }
+          k = p;
         }
-        k = p;
+        if ((j >> 5) >= words && a.err_flag) atomicOr(a.err_flag, TQ4_DEV_BAD_TREE);  // (its own bit has no room)
       }
-      if (j >= 32ll * a.words && w == 0 && a.err_flag) atomicOr(a.err_flag, TQ4_DEV_BAD_TREE);  // (its own bit has no room)
+      a.depth[r0 + j] = depth;
     }
-    a.mask[r0 * a.words + i] = (int32_t)bits;
-    if (w == 0) a.depth[r0 + j] = depth;
+    __syncthreads();
+    int32_t* out = a.mask + (r0 + b0) * words;
+    for (int i = tid; i < rows * words; i += kMaskThreads) {
+      const int row = i / words;
+      out[i] = (int32_t)s_bits[row * pitch + (i - row * words)];
+    }
+    __syncthreads();
   }
 }
 
@@ -74,12 +77,18 @@ extern "C" int tq4_tree_mask(const int32_t* parents, const int32_t* query_start_
   if (num_rows < 0 || num_rows > 0x7fffffff || num_seqs < 0 || words <= 0) return TQ4_ERR_INVALID_ARG;
   if (num_rows == 0) return TQ4_OK;
   if (!parents || !query_start_loc || !mask || !depth) return TQ4_ERR_INVALID_ARG;
-  const MaskArgs a{parents, query_start_loc, num_rows, num_seqs, words, mask, depth, err_flag};
-  // (an even share of the words for every block, as if the sequences were alike)
-  const int64_t items = (num_rows * words + num_seqs) / (num_seqs > 0 ? num_seqs : 1);
-  int64_t shares = (items + kMaskThreads - 1) / kMaskThreads;
+  MaskArgs a{parents, query_start_loc, num_rows, num_seqs, words, 0, mask, depth, err_flag};
+  // as many rows as there are threads, where their words fit
+  const int row_bytes = (words | 1) * 4;
+  a.block_rows = kMaskBytes / row_bytes < kMaskThreads ? kMaskBytes / row_bytes : kMaskThreads;
+  if (a.block_rows < 1) return TQ4_ERR_UNSUPPORTED;
+  if ((int64_t)a.block_rows > num_rows) a.block_rows = (int)num_rows;
+  const int smem = a.block_rows * row_bytes;
+  if (!ensure_dynamic_smem<tree_mask_kernel>(kMaskBytes)) return TQ4_ERR_CUDA;
+  // (blocks for sequences of as many drafts as there are bits)
+  int64_t shares = (32 * (int64_t)words + a.block_rows - 1) / a.block_rows;
   if (shares > 64) shares = 64;
-  if (launch_kernel(tree_mask_kernel, dim3((unsigned)num_seqs + 1, (unsigned)shares), dim3(kMaskThreads), 0, (cudaStream_t)stream, false,
+  if (launch_kernel(tree_mask_kernel, dim3((unsigned)num_seqs + 1, (unsigned)shares), dim3(kMaskThreads), (size_t)smem, (cudaStream_t)stream, false,
                     a) != cudaSuccess)
     return TQ4_ERR_CUDA;
   TQ4_CHECK_LAUNCH();
