@@ -160,6 +160,10 @@ CASES = [  # head_dim, q heads, KV heads, lengths, drafts, block size, window, r
     (128, 8, 4, [500, 100, 20], [20, 33, 20], 16, 48, True, "bf16"),     # a window
     (128, 8, 4, [500, 100], [20, 70], 16, 3, True, "bf16"),              # ... shorter than the branches
     (128, 8, 8, [90], [40], 16, None, True, "fp32"),
+    (128, 32, 8, [3000, 70], [30, 3], 16, None, True, "bf16"),           # few drafts, cut along the keys
+    (128, 2, 2, [130], [40], 48, None, True, "bf16"),                    # rows whose values start on 8 bytes; pages of three boxes
+    (64, 3, 3, [100, 257], [5, 40], 16, 100, False, "fp16"),             # ... rows of 216 bytes
+    (96, 8, 1, [77], [16], 16, None, True, "bf16"),
 ]
 DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
 
@@ -173,7 +177,9 @@ def _call(ops, q, case, nodes, mask, p, hkv, bs, **kw):
 def _check(got, lse, want, want_lse, spread, out_dtype=torch.float32):
     # Keys and values are centroids on the tensor cores' fp16 grid (half a step: 2^-11 of the value); an error of 2^-11 in a key moves
     # its score, and with it its weight, by 2^-11 of the score.  16-bit outputs add half a step of their own.
-    tol = 2 ** -11 * (1 + spread) + (0 if out_dtype == torch.float32 else torch.finfo(out_dtype).eps / 2)
+    # Calls with a bf16 output may round queries and weights to fp16 as well (2^-11 of the score, and of the weight, once more).
+    tol = 2 ** -11 * (1 + spread) * (2 if out_dtype == torch.bfloat16 else 1)
+    tol += 0 if out_dtype == torch.float32 else torch.finfo(out_dtype).eps / 2
     assert torch.isfinite(got).all()
     assert (got.double() - want).norm() <= tol * want.norm() + 1e-30
     if lse is not None:
@@ -195,6 +201,9 @@ def test_tree_attention(ops, d, hq, hkv, lens, nodes, bs, window, padded, dtype)
                 out_dtype=torch.float32, lse_out=lse)
     want, want_lse, spread = reference(q, case, nodes, matrices, pr, hkv, bs, d ** -0.5, window)
     _check(got.cpu(), lse.cpu(), want, want_lse, spread)
+    for out_dtype in (torch.bfloat16, torch.float16):
+        got = _call(ops, q, case, nodes, pack(matrices, -(-max(nodes) // 32)), pr.cuda(), hkv, bs, sliding_window=window, out_dtype=out_dtype)
+        _check(got.cpu(), None, want, None, spread, out_dtype)
     assert ops.read_and_clear_errors(got.device) == 0
 
 
@@ -272,7 +281,8 @@ def test_16bit_output_strided_queries_and_rows_behind_the_last_sequence(ops, dty
                                        mask.cuda(), p["kc"], p["vc"], p["rot"], 2, 16, out=out[..., :128])
     assert got.data_ptr() == out.data_ptr() and (out[..., 128:] == 7).all()
     full = _call(ops, fused[:, :8].contiguous(), case, nodes, mask, p, 2, 16, out_dtype=torch.float32)
-    assert torch.equal(out[..., :128], full.to(out.dtype))
+    if dtype == "fp16":  # (the rounded fp32 output; a bf16 output's queries and weights are rounded, too)
+        assert torch.equal(out[..., :128], full.to(out.dtype))
     want, want_lse, spread = reference(fused[:14, :8], case, nodes, matrices, pr, 2, 16, 128 ** -0.5)
     _check(out[:14, :, :128].cpu(), None, want, want_lse, spread, DTYPES[dtype])
     assert (out[14:, :, :128] == 0).all()

@@ -99,7 +99,8 @@ extern "C" size_t tq4_tree_attention_workspace_bytes(int64_t max_query_rows, int
   using namespace tq4;
   AttnShape sh{};
   if (max_query_rows <= 0 || !supported_head_dim(head_dim) || !make_shape(sh, num_q_heads, num_kv_heads, head_dim) || sh.G > 128) return 0;
-  int64_t vectors = 32 * max_query_rows * num_q_heads;
+  // (parts only where the rows leave SMs idle: two CTAs of 128 rows each an SM)
+  int64_t vectors = 64 * max_query_rows * num_q_heads;
   if (vectors > kPrefillSplitVectors) vectors = kPrefillSplitVectors;
   // (a vector set of Hq and the alignment of the image on top: tree_tc_splits counts whole sets)
   return 128 + prefill_tc_image_bytes(head_dim) + (size_t)(vectors + num_q_heads) * (head_dim + 1) * 4;
@@ -173,11 +174,16 @@ extern "C" int tq4_tree_attention(
   uint8_t* image = reinterpret_cast<uint8_t*>(((uintptr_t)workspace + 127) & ~(uintptr_t)127);
   float* part_o = reinterpret_cast<float*>(image + prefill_tc_image_bytes(head_dim));
   const int64_t room = (int64_t)((uintptr_t)workspace + workspace_bytes) - (int64_t)(uintptr_t)part_o;
-  const int splits = tree_tc_splits(a, room / ((int64_t)num_q_heads * (head_dim + 1) * 4) - 1);
+  // The kernel for few drafts takes 128 / G rows of a sequence a CTA, the other twice that: the first, unless sequences fill more than one of
+  // its CTAs on average, which would dequantise every tile again.
+  const bool few = tree_few_supported(a) && num_rows * a.sh.G <= 128 * (int64_t)(num_seqs > 0 ? num_seqs : 1);
+  const int64_t slots = room / ((int64_t)num_q_heads * (head_dim + 1) * 4) - 1;
+  const int splits = few ? tree_few_splits(a, slots) : tree_tc_splits(a, slots);
   const bool to_parts = splits > 1;
   float* part_m = part_o + (size_t)splits * num_rows * num_q_heads * head_dim;
   prof_begin(TQ4_PROF_ATTENTION, st);
-  const int rc = launch_tree_tc(a, st, splits, to_parts, image, part_o, part_m);
+  const int rc = few ? launch_tree_few(a, st, splits, to_parts, image, part_o, part_m)
+                     : launch_tree_tc(a, st, splits, to_parts, image, part_o, part_m);
   prof_end(TQ4_PROF_ATTENTION, st);
   if (rc != TQ4_OK || !to_parts) return rc;
   CombineArgs c{};
