@@ -216,7 +216,7 @@ int tree_tc_splits(const AttnArgs& a, int64_t slots);
 // ... and its sibling for sequences of few drafts (tq4_tree_tc.cu)
 int launch_pi_image(int D, const float* rotation, uint8_t* image, cudaStream_t st);
 bool tree_few_supported(const AttnArgs& a);
-int tree_few_splits(const AttnArgs& a, int64_t slots);
+int tree_few_splits(const AttnArgs& a, int64_t room);
 int launch_tree_few(const AttnArgs& a, cudaStream_t st, int splits, bool to_parts, uint8_t* image, float* part_o, float* part_m);
 int launch_tree_tc(const AttnArgs& a, cudaStream_t st, int splits, bool to_parts, uint8_t* image, float* part_o, float* part_m);
 constexpr int kPrefillMinRows = 8;  // new rows of a sequence from which the prefill kernel is the faster one

@@ -30,6 +30,7 @@ constexpr int kSmx = 128, kDeq = 128;
 constexpr int kThreads = kSmx + kDeq + 64;
 constexpr int kIssueWarp = (kSmx + kDeq) / 32, kFetchWarp = kIssueWarp + 1;
 constexpr int kGroup = 16;  // tokens of a box
+constexpr int kMinTiles = 2;  // of a key part
 
 template <int D, bool FAST>
 struct Cfg {
@@ -43,9 +44,10 @@ struct Cfg {
   static constexpr uint32_t kCols = 256;
   static_assert(kColO + D <= kCols, "tensor memory");
   // shared memory, from a 1024-byte boundary
-  static constexpr uint32_t kKv = NC * kBN * 128;          // K~ or V~
+  static constexpr uint32_t kKv = NC * kBN * 128;          // K~ or V~ of a tile
+  static constexpr int NVB = QLO_SMEM ? 1 : 2;             // V~ buffers, where there is room: values are written while the tile before is in its softmax
   static constexpr uint32_t kImgPart = D * 128, kImgTerm = NC * kImgPart;  // Pi's image: its hi term shares K~ and V~, its lo term the tables
-  static constexpr uint32_t kOffK = 0, kOffV = kKv, kOffLut = 2 * kKv, kLut = 32768;
+  static constexpr uint32_t kOffK = 0, kOffV = kKv, kOffLut = (1 + NVB) * kKv, kLut = 32768;
   static_assert(kImgTerm <= 2 * kKv && kImgTerm <= kLut, "room for Pi's image");
   static constexpr uint32_t kOffQlo = kOffLut + kLut;
   static constexpr uint32_t kOffRaw = kOffQlo + (QLO_SMEM ? NC * 128 * 128 : 0);
@@ -66,7 +68,8 @@ struct Cfg {
 
 struct TreeArgs {
   const uint8_t* image;  // Pi's operand image
-  int splits;            // parts of the key range
+  int splits;            // key parts of a row, at most
+  int slots;             // CTAs of a KV head that the parts are cut for
   int to_parts;          // leave partials for the merge kernel instead of writing the output
   float* part_o;         // [splits][rows][Hq][D] normalised, rotated
   float* part_m;         // [splits][rows][Hq] natural-log LSE
@@ -75,8 +78,8 @@ struct TreeArgs {
 struct Bars {
   uint64_t rawk[2], rawv[2];          // packed keys and norms / values of a stage landed
   uint64_t rawk_free[2], rawv_free[2];  // ... and read
-  uint64_t kready, vready;            // dequantising warps -> issuer: K~ / V~ written
-  uint64_t kfree, vfree;              // MMAs -> dequantising warps: K~ / V~ read
+  uint64_t kready, vready[2];         // dequantising warps -> issuer: K~ / V~ (of a buffer) written
+  uint64_t kfree, vfree[2];           // MMAs -> dequantising warps: ... read
   uint64_t sready, pready;            // MMAs -> softmax: scores complete / softmax -> issuer: P written
   uint64_t img, aready, rot, qready;  // Pi's image landed / A operand of a rotation staged / rotation complete / queries in place
   uint64_t odone, drain;              // last MMA of the tile loop / of a dead CTA complete
@@ -85,6 +88,44 @@ struct Bars {
 __device__ __forceinline__ void box_load(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
   asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
                ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
+}
+
+// Rows [q0, q1) of sequence s, n blocks of RB of them; its length, and the t tiles of keys that they see.
+__device__ __forceinline__ void sequence_shape(const AttnArgs& a, int RB, int s, int& q0, int& q_end, int& q1, int& seq_len, int& n, int& t) {
+  q0 = q_end = q1 = seq_len = n = t = 0;
+  if (s >= a.sh.num_seqs) return;
+  q0 = max(__ldg(a.query_start_loc + s), 0);
+  q_end = __ldg(a.query_start_loc + s + 1);
+  q1 = min(q_end, a.sh.rows);
+  seq_len = __ldg(a.seq_lens + s);
+  n = q1 > q0 ? (q1 - q0 + RB - 1) / RB : 0;
+  const int len = (int)min((long long)max(seq_len, 0), (long long)a.table_width * a.block_size), held = len - (q_end - q0);
+  const int lo = a.sliding_window > 0 ? min(max(0, held - a.sliding_window), len) : 0;
+  t = len > lo ? (len - lo / kBN * kBN + kBN - 1) / kBN : 0;
+}
+
+// The fewest tiles a key part with which all parts of a KV head find a slot at once (a warp; out of the way of the code that is run often).
+__device__ __noinline__ int tiles_per_part(const AttnArgs& a, const TreeArgs& pa, int RB, int lane) {
+  int n0, t0, x0, x1, x2, x3, longest = 0;
+  sequence_shape(a, RB, lane, x0, x1, x2, x3, n0, t0);  // (the first 32 sequences stay in registers)
+  for (int s0 = 0; s0 < a.sh.num_seqs; s0 += 32) {
+    int n = n0, t = t0;
+    if (s0 > 0) sequence_shape(a, RB, s0 + lane, x0, x1, x2, x3, n, t);
+    longest = max(longest, __reduce_max_sync(0xffffffffu, n > 0 ? t : 0));
+  }
+  int lo = max(kMinTiles, (longest + pa.splits - 1) / pa.splits), hi = max(lo, longest);
+  while (lo < hi) {
+    const int mid = (lo + hi) / 2;
+    int parts = 0;
+    for (int s0 = 0; s0 < a.sh.num_seqs; s0 += 32) {
+      int n = n0, t = t0;
+      if (s0 > 0) sequence_shape(a, RB, s0 + lane, x0, x1, x2, x3, n, t);
+      parts += __reduce_add_sync(0xffffffffu, n * max(1, (t + mid - 1) / mid));
+    }
+    if (parts <= pa.slots) hi = mid;
+    else lo = mid + 1;
+  }
+  return lo;
 }
 
 template <int D, bool FAST>
@@ -96,7 +137,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   __shared__ __align__(8) Bars s_bars;
   __shared__ uint32_t s_tmem;
-  __shared__ int s_info[6];        // sequence, first row and rows of the CTA; end of the sequence's rows, its length, their start
+  __shared__ int s_info[8];        // sequence, first row and rows of the CTA; end of the sequence's rows, its length, their start; key part, parts
   __shared__ float s_cent[2][16];  // scaled centroids of K and V
   __shared__ int s_dead, s_bad;    // a wait gave up / some page id is out of range
   __shared__ int s_badgrp[2];      // groups of the stage's tile whose page id is
@@ -108,20 +149,18 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
   const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u;
   unsigned char* sm = smem_raw + (base - smem_addr(smem_raw));
 
-  // ---- which rows are this CTA's? ----------------------------------------------------------------------------
+  // ---- which rows and keys are this CTA's? -----------------------------------------------------------------------
+  // A sequence's rows make n blocks of RB rows, its keys t tiles; in a call cut along the keys every block has ceil(t / per) parts, with
+  // the fewest tiles a part, `per`, for which all parts find a slot at once: long sequences are cut into more.  (As many parts for all of
+  // them: 16 of 300 to 8100 tokens 157 us, 115 so.)
   if (warp == 0) {
+    const int per = pa.to_parts ? tiles_per_part(a, pa, RB, lane) : 0x3fffffff;
     int acc = 0, found = -1, first = 0, nrows = 0;
     for (int s0 = 0; s0 < sh.num_seqs && found < 0; s0 += 32) {
-      const int s = s0 + lane;
-      int q0 = 0, q1 = 0, q_end = 0, seq_len = 0;
-      if (s < sh.num_seqs) {
-        q0 = max(__ldg(a.query_start_loc + s), 0);
-        q_end = __ldg(a.query_start_loc + s + 1);
-        seq_len = __ldg(a.seq_lens + s);
-        q1 = min(q_end, sh.rows);
-      }
-      const int n = q1 > q0 ? (q1 - q0 + RB - 1) / RB : 0;
-      int incl = n;
+      int q0, q_end, q1, seq_len, n, t;
+      sequence_shape(a, RB, s0 + lane, q0, q_end, q1, seq_len, n, t);
+      const int parts = max(1, (t + per - 1) / per), c = n * parts;
+      int incl = c;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int up = __shfl_up_sync(0xffffffffu, incl, o);
@@ -131,7 +170,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
       const unsigned m = __ballot_sync(0xffffffffu, x < incl);
       if (m) {
         const int w = __ffs(m) - 1;
-        const int b = x - (incl - n);  // (lane w: its block)
+        const int at = x - (incl - c), b = at / parts;  // (lane w: its block)
         found = s0 + w;
         first = __shfl_sync(0xffffffffu, q0 + b * RB, w);
         nrows = __shfl_sync(0xffffffffu, min(RB, q1 - (q0 + b * RB)), w);
@@ -139,6 +178,8 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
           s_info[3] = q_end;
           s_info[4] = seq_len;
           s_info[5] = q0;
+          s_info[6] = at - b * parts;
+          s_info[7] = parts;
         }
       }
       acc += __shfl_sync(0xffffffffu, incl, 31);
@@ -170,7 +211,8 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
         if (!pa.to_parts)
           store4(a.out, a.out_dtype, (int64_t)r * a.out_token_stride + (int64_t)h * a.out_head_stride + d, zero);
         if (d > 0) continue;
-        if (pa.to_parts) pa.part_m[((int64_t)blockIdx.y * sh.rows + r) * sh.Hq + h] = -CUDART_INF_F;
+        if (pa.to_parts)
+          for (int p = 0; p < pa.splits; ++p) pa.part_m[((int64_t)p * sh.rows + r) * sh.Hq + h] = -CUDART_INF_F;
         else if (a.lse_out) a.lse_out[(int64_t)r * sh.Hq + h] = -CUDART_INF_F;
       }
     }
@@ -183,11 +225,11 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
       bar_init(bar(s_bars.rawv[i]), 1);
       bar_init(bar(s_bars.rawk_free[i]), kDeq / 32);
       bar_init(bar(s_bars.rawv_free[i]), kDeq / 32);
+      bar_init(bar(s_bars.vready[i]), kDeq / 32);
+      bar_init(bar(s_bars.vfree[i]), 1);
     }
     bar_init(bar(s_bars.kready), kDeq / 32);
-    bar_init(bar(s_bars.vready), kDeq / 32);
     bar_init(bar(s_bars.kfree), 1);
-    bar_init(bar(s_bars.vfree), 1);
     bar_init(bar(s_bars.sready), 1);
     bar_init(bar(s_bars.pready), row_warps);
     bar_init(bar(s_bars.img), 1);
@@ -205,6 +247,13 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
   }
   pdl_trigger();
   pdl_wait();  // the operand image of Pi; everything else was complete before the kernel in front started
+  if (pa.to_parts && s_info[6] == 0) {  // the parts that these rows do not have
+    const int parts = s_info[7];
+    for (int i = tid; i < (pa.splits - parts) * nrows * G; i += kThreads) {
+      const int p = i / (nrows * G), r = i - p * (nrows * G);
+      pa.part_m[((int64_t)(parts + p) * sh.rows + row0 + r / G) * sh.Hq + kvh * G + r % G] = -CUDART_INF_F;
+    }
+  }
   fence_before();
   __syncthreads();
   fence_after();
@@ -218,9 +267,9 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
     if (len > lo) {
       t_first = lo / kBN * kBN;
       n_tiles = (len - t_first + kBN - 1) / kBN;
-      const int per = (n_tiles + pa.splits - 1) / pa.splits;  // this part of the key range
-      t_first += (int)blockIdx.y * per * kBN;
-      n_tiles = max(0, min(per, n_tiles - (int)blockIdx.y * per));
+      const int part = s_info[6], parts = s_info[7], per = (n_tiles + parts - 1) / parts;  // this part of the key range
+      t_first += part * per * kBN;
+      n_tiles = max(0, min(per, n_tiles - part * per));
     }
   }
   const RowLayout lay = row_layout(sh.Hkv, D);
@@ -330,12 +379,12 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
       auto issue_pv = [&](int j) {  // O += P V~
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
-          const uint64_t dv = d_v + (uint64_t)((2048 * s) >> 4);
+          const uint64_t dv = d_v + (uint64_t)(((j % C::NVB) * C::kKv + 2048 * s) >> 4);
           const uint32_t ph = tmem + C::kColS + 16 * s;
           if (!FAST) mma_ta(tmem + C::kColO, ph + 8, dv, idO, j > 0 || s > 0);
           mma_ta(tmem + C::kColO, ph, dv, idO, !FAST || j > 0 || s > 0);
         }
-        mma_commit(bar(s_bars.vfree));
+        mma_commit(bar(s_bars.vfree[j % C::NVB]));
       };
       ok = ok && bar_wait(bar(s_bars.qready), 0u, dead);
       ok = ok && bar_wait(bar(s_bars.kready), 0u, dead);
@@ -344,7 +393,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
         issue_s();
       }
       for (int j = 0; j < n_tiles && ok; ++j) {
-        ok = bar_wait(bar(s_bars.vready), (uint32_t)(j & 1), dead) && bar_wait(bar(s_bars.pready), (uint32_t)(j & 1), dead);
+        ok = bar_wait(bar(s_bars.vready[j % C::NVB]), (uint32_t)((j / C::NVB) & 1), dead) && bar_wait(bar(s_bars.pready), (uint32_t)(j & 1), dead);
         if (!ok) break;
         fence_after();
         issue_pv(j);
@@ -405,9 +454,8 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
       }
     }
     asm volatile("bar.sync 1, %0;" ::"n"(kDeq) : "memory");
-    const int shift = one_table ? 7 : 6;
-    const uint32_t lut_mask = 255u << shift;
-    const uint32_t lut_k = base + C::kOffLut + (lane & ((1 << (shift - 2)) - 1)) * 4, lut_v = lut_k + (one_table ? 0u : 256u << shift);
+    const uint32_t entry = one_table ? 128 : 64;  // bytes of a byte's copies
+    const uint32_t lut_k = base + C::kOffLut + (lane & (entry / 4 - 1)) * 4, lut_v = lut_k + (one_table ? 0u : 256 * entry);
     auto look = [&](uint32_t at) -> uint32_t {
       uint32_t y;
       asm volatile("ld.shared.b32 %0, [%1];" : "=r"(y) : "r"(at));
@@ -419,8 +467,8 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         const uint32_t x = w[c];
-        const uint4 o = make_uint4(look(lut + ((x << shift) & lut_mask)), look(lut + ((x >> (8 - shift)) & lut_mask)),
-                                   look(lut + ((x >> (16 - shift)) & lut_mask)), look(lut + ((x >> (24 - shift)) & lut_mask)));
+        const uint4 o = make_uint4(look(lut + __byte_perm(x, 0u, 0x4440) * entry), look(lut + __byte_perm(x, 0u, 0x4441) * entry),
+                                   look(lut + __byte_perm(x, 0u, 0x4442) * entry), look(lut + (x >> 24) * entry));
         *reinterpret_cast<uint4*>(dst + swz(tok, (seg & 1) * 4 + c)) = o;
       }
     };
@@ -457,7 +505,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
       done(s_bars.kready, s_bars.rawk_free[st]);
       // ---- values ----------------------------------------------------------------------------------------------
       ok = bar_wait(bar(s_bars.rawv[st]), (uint32_t)(u & 1), dead);
-      if (j > 0) ok = ok && bar_wait(bar(s_bars.vfree), (uint32_t)((j - 1) & 1), dead);
+      if (j >= C::NVB) ok = ok && bar_wait(bar(s_bars.vfree[j % C::NVB]), (uint32_t)((j / C::NVB - 1) & 1), dead);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
 #pragma unroll
@@ -472,10 +520,10 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             const uint32_t* w = reinterpret_cast<const uint32_t*>(p);
             x = make_uint4(w[0], w[1], w[2], w[3]);
           }
-          expand(x, lut_v, C::kOffV, tok, seg);
+          expand(x, lut_v, C::kOffV + (j % C::NVB) * C::kKv, tok, seg);
         }
       }
-      done(s_bars.vready, s_bars.rawv_free[st]);
+      done(s_bars.vready[j % C::NVB], s_bars.rawv_free[st]);
     }
   } else {
     // ================= softmax warps: a row per thread =================
@@ -584,10 +632,11 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
         // dot x key norm x qscale - reference, exp2, x value norm, (split,) store in place; two columns per instruction.  The reference is updated
         // lazily, and looked at only after the fact: when some weight exceeds 2^8 (or the row has no reference yet) the tile is done
         // again from the scores, which stay in registers, with a new one.
+        const int any_bad = *(volatile int*)&s_bad;  // (its latency beside the scores')
         uint32_t v[kBN];
         tmem_ld_cols(scol, v);
         bool seen = true;  // some key of the tile is visible
-        if (!__all_sync(0xffffffffu, t0 >= kv_lo && kv_hi - kBN >= t0 && qexp == 1.f) || *(volatile int*)&s_bad) {
+        if (!__all_sync(0xffffffffu, t0 >= kv_lo && kv_hi - kBN >= t0 && qexp == 1.f) || any_bad) {
           // hidden columns: a score of -inf (key norms are positive in shared memory)
           const int lo = min(max(kv_lo - t0, 0), kBN), hi = min(max(kv_hi - t0, 0), kBN);
           uint32_t vis[2];
@@ -600,7 +649,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
               const int k = t0 + 32 * w - held, n = min(max(len - (t0 + 32 * w), 0), 32);
               if (n > 0 && k > -32) vis[w] |= draft_bits(k) & (0xFFFFFFFFu >> (32 - n));
             }
-            if (*(volatile int*)&s_bad)
+            if (any_bad)
               for (int i = 0; i < 32; ++i)
                 if (ns[32 * w + i] == kHidden) vis[w] &= ~(1u << i);
             seen = seen || vis[w];
@@ -734,7 +783,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
         }
       };
       if (pa.to_parts || a.out_rotated) {
-        const int64_t vec = ((int64_t)blockIdx.y * sh.rows + row) * sh.Hq + head;
+        const int64_t vec = ((int64_t)s_info[6] * sh.rows + row) * sh.Hq + head;
 #pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
           uint32_t v[32];
@@ -828,9 +877,11 @@ int launch_t(const AttnArgs& a, const TreeArgs& pa, cudaStream_t st) {
   CUtensorMap mk, mv, mn;
   if (!cache_map(mk, a, D / 2) || !cache_map(mv, a, C::kVPitch) || !cache_map(mn, a, 16)) return TQ4_ERR_CUDA;
   const int per_cta = 128 / a.sh.G;
-  const int64_t grid = ((int64_t)(a.sh.rows + per_cta - 1) / per_cta + a.sh.num_seqs) * a.sh.Hkv;  // upper bound
+  int64_t units = (int64_t)(a.sh.rows + per_cta - 1) / per_cta + a.sh.num_seqs;  // upper bound, with one spare
+  if (pa.to_parts && units < pa.slots + 1) units = pa.slots + 1;
+  const int64_t grid = units * a.sh.Hkv;
   if (grid > 0x7fffffff) return TQ4_ERR_UNSUPPORTED;
-  if (launch_kernel(tree_tc_kernel<D, FAST>, dim3((unsigned)grid, (unsigned)pa.splits), dim3(kThreads), (size_t)smem, st, true, mk, mv, mn, a,
+  if (launch_kernel(tree_tc_kernel<D, FAST>, dim3((unsigned)grid), dim3(kThreads), (size_t)smem, st, true, mk, mv, mn, a,
                     pa) != cudaSuccess)
     return TQ4_ERR_CUDA;
   TQ4_CHECK_LAUNCH();
@@ -845,20 +896,28 @@ bool tree_few_supported(const AttnArgs& a) {
          a.cache_token_stride <= (1 << 30) && a.cache_block_stride >= a.cache_token_stride && encode_tiled_fn() != nullptr;
 }
 
-// Key parts: as many as give every SM its two CTAs.
-int tree_few_splits(const AttnArgs& a, int64_t slots) {
+// CTAs of a KV head that run at once, two an SM.
+int tree_few_slots(const AttnArgs& a) {
+  const int s = 2 * sm_count() / a.sh.Hkv;
+  return s < 1 ? 1 : s;
+}
+
+// Key parts of a row, at most: none where the sequences fill the SMs already.
+int tree_few_splits(const AttnArgs& a, int64_t room) {
   const int per_cta = 128 / a.sh.G;
-  const int64_t blocks = (a.sh.rows + per_cta - 1) / per_cta, ctas = (blocks > a.sh.num_seqs ? blocks : a.sh.num_seqs) * a.sh.Hkv;
-  int64_t s = 2 * (int64_t)sm_count() / (ctas > 0 ? ctas : 1);
-  const int64_t keys = a.sliding_window > 0 && a.sliding_window + kBN < a.max_keys ? a.sliding_window + kBN : a.max_keys, tiles = keys / kBN;
-  if (s > tiles / 4) s = tiles / 4;
+  const int64_t blocks = (a.sh.rows + per_cta - 1) / per_cta, units = blocks > a.sh.num_seqs ? blocks : a.sh.num_seqs;
+  int64_t s = tree_few_slots(a);
+  if (5 * units > 4 * s) return 1;  // (hardly any sequence would be cut, and all would go through the merge)
+  const int64_t keys = a.sliding_window > 0 && a.sliding_window + kBN < a.max_keys ? a.sliding_window + kBN : a.max_keys;
+  const int64_t tiles = (keys + kBN - 1) / kBN + 1;
+  if (s > tiles / kMinTiles) s = tiles / kMinTiles;
   if (s > 64) s = 64;
-  if (a.sh.rows > 0 && s > slots / a.sh.rows) s = slots / a.sh.rows;
+  if (a.sh.rows > 0 && s > room / a.sh.rows) s = room / a.sh.rows;
   return s < 1 ? 1 : (int)s;
 }
 
 int launch_tree_few(const AttnArgs& a, cudaStream_t st, int splits, bool to_parts, uint8_t* image, float* part_o, float* part_m) {
-  const TreeArgs pa{image, splits, to_parts ? 1 : 0, part_o, part_m};
+  const TreeArgs pa{image, splits, tree_few_slots(a), to_parts ? 1 : 0, part_o, part_m};
   const int rc = launch_pi_image(a.sh.D, a.rotation, image, st);
   if (rc != TQ4_OK) return rc;
   const bool fast = a.out_dtype == TQ4_BF16;
