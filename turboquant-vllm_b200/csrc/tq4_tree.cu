@@ -198,7 +198,7 @@ extern "C" int tq4_tree_attention(
   c.out_token_stride = out_token_stride;
   c.out_head_stride = out_head_stride;
   c.lse_out = lse_out;
-  c.out_rotated = out_rotated;
+  c.out_rotated = few || out_rotated;  // (that kernel's parts are un-rotated already)
   prof_begin(TQ4_PROF_COMBINE, st);
   const int rc2 = launch_combine(c, head_dim, st, true);
   prof_end(TQ4_PROF_COMBINE, st);

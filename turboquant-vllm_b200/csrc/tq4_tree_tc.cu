@@ -46,7 +46,9 @@ struct Cfg {
   // shared memory, from a 1024-byte boundary
   static constexpr uint32_t kKv = NC * kBN * 128;          // K~ or V~ of a tile
   static constexpr int NVB = QLO_SMEM ? 1 : 2;             // V~ buffers, where there is room: values are written while the tile before is in its softmax
-  static constexpr uint32_t kImgPart = D * 128, kImgTerm = NC * kImgPart;  // Pi's image: its hi term shares K~ and V~, its lo term the tables
+  // Pi's image.  Rotation: its hi term where K~ and V~ come to lie, its lo term (not FAST) where the tables do.  Un-rotation: the hi term in place of
+  // the tables, which are read for the last time before the last weights are there, the lo term in place of K~ and V~.
+  static constexpr uint32_t kImgPart = D * 128, kImgTerm = NC * kImgPart;
   static constexpr uint32_t kOffK = 0, kOffV = kKv, kOffLut = (1 + NVB) * kKv, kLut = 32768;
   static_assert(kImgTerm <= 2 * kKv && kImgTerm <= kLut, "room for Pi's image");
   static constexpr uint32_t kOffQlo = kOffLut + kLut;
@@ -71,7 +73,7 @@ struct TreeArgs {
   int splits;            // key parts of a row, at most
   int slots;             // CTAs of a KV head that the parts are cut for
   int to_parts;          // leave partials for the merge kernel instead of writing the output
-  float* part_o;         // [splits][rows][Hq][D] normalised, rotated
+  float* part_o;         // [splits][rows][Hq][D] normalised, in the output's space
   float* part_m;         // [splits][rows][Hq] natural-log LSE
 };
 
@@ -90,27 +92,35 @@ __device__ __forceinline__ void box_load(uint32_t dst, const CUtensorMap* map, i
                ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
 }
 
-// Rows [q0, q1) of sequence s, n blocks of RB of them; its length, and the t tiles of keys that they see.
-__device__ __forceinline__ void sequence_shape(const AttnArgs& a, int RB, int s, int& q0, int& q_end, int& q1, int& seq_len, int& n, int& t) {
-  q0 = q_end = q1 = seq_len = n = t = 0;
-  if (s >= a.sh.num_seqs) return;
-  q0 = max(__ldg(a.query_start_loc + s), 0);
-  q_end = __ldg(a.query_start_loc + s + 1);
-  q1 = min(q_end, a.sh.rows);
-  seq_len = __ldg(a.seq_lens + s);
-  n = q1 > q0 ? (q1 - q0 + RB - 1) / RB : 0;
-  const int len = (int)min((long long)max(seq_len, 0), (long long)a.table_width * a.block_size), held = len - (q_end - q0);
+// A sequence: its rows [q0, q1) (q_end before the call's rows cut them), n blocks of RB of them; its length, and the t tiles of keys they see.
+struct SeqShape {
+  int q0, q_end, q1, seq_len, n, t;
+};
+__device__ __forceinline__ SeqShape sequence_shape(const AttnArgs& a, int RB, int s) {
+  SeqShape x{0, 0, 0, 0, 0, 0};
+  if (s >= a.sh.num_seqs) return x;
+  x.q0 = max(__ldg(a.query_start_loc + s), 0);
+  x.q_end = __ldg(a.query_start_loc + s + 1);
+  x.seq_len = __ldg(a.seq_lens + s);
+  x.q1 = min(x.q_end, a.sh.rows);
+  x.n = x.q1 > x.q0 ? (x.q1 - x.q0 + RB - 1) / RB : 0;
+  const int len = (int)min((long long)max(x.seq_len, 0), (long long)a.table_width * a.block_size), held = len - (x.q_end - x.q0);
   const int lo = a.sliding_window > 0 ? min(max(0, held - a.sliding_window), len) : 0;
-  t = len > lo ? (len - lo / kBN * kBN + kBN - 1) / kBN : 0;
+  x.t = len > lo ? (len - lo / kBN * kBN + kBN - 1) / kBN : 0;
+  return x;
 }
 
-// The fewest tiles a key part with which all parts of a KV head find a slot at once (a warp; out of the way of the code that is run often).
-__device__ __noinline__ int tiles_per_part(const AttnArgs& a, const TreeArgs& pa, int RB, int lane) {
-  int n0, t0, x0, x1, x2, x3, longest = 0;
-  sequence_shape(a, RB, lane, x0, x1, x2, x3, n0, t0);  // (the first 32 sequences stay in registers)
+// The fewest tiles a key part with which all parts of a KV head find a slot at once (a warp; `x`: the lane's sequence of the first 32; out of
+// the way of the code that is run often).
+__device__ __noinline__ int tiles_per_part(const AttnArgs& a, const TreeArgs& pa, int RB, int lane, int n0, int t0) {
+  int longest = 0;
   for (int s0 = 0; s0 < a.sh.num_seqs; s0 += 32) {
     int n = n0, t = t0;
-    if (s0 > 0) sequence_shape(a, RB, s0 + lane, x0, x1, x2, x3, n, t);
+    if (s0 > 0) {
+      const SeqShape x = sequence_shape(a, RB, s0 + lane);
+      n = x.n;
+      t = x.t;
+    }
     longest = max(longest, __reduce_max_sync(0xffffffffu, n > 0 ? t : 0));
   }
   int lo = max(kMinTiles, (longest + pa.splits - 1) / pa.splits), hi = max(lo, longest);
@@ -119,7 +129,11 @@ __device__ __noinline__ int tiles_per_part(const AttnArgs& a, const TreeArgs& pa
     int parts = 0;
     for (int s0 = 0; s0 < a.sh.num_seqs; s0 += 32) {
       int n = n0, t = t0;
-      if (s0 > 0) sequence_shape(a, RB, s0 + lane, x0, x1, x2, x3, n, t);
+      if (s0 > 0) {
+        const SeqShape x = sequence_shape(a, RB, s0 + lane);
+        n = x.n;
+        t = x.t;
+      }
       parts += __reduce_add_sync(0xffffffffu, n * max(1, (t + mid - 1) / mid));
     }
     if (parts <= pa.slots) hi = mid;
@@ -154,30 +168,30 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
   // the fewest tiles a part, `per`, for which all parts find a slot at once: long sequences are cut into more.  (As many parts for all of
   // them: 16 of 300 to 8100 tokens 157 us, 115 so.)
   if (warp == 0) {
-    const int per = pa.to_parts ? tiles_per_part(a, pa, RB, lane) : 0x3fffffff;
+    const SeqShape own = sequence_shape(a, RB, lane);
+    const int per = pa.to_parts ? tiles_per_part(a, pa, RB, lane, own.n, own.t) : 0x3fffffff;
     int acc = 0, found = -1, first = 0, nrows = 0;
     for (int s0 = 0; s0 < sh.num_seqs && found < 0; s0 += 32) {
-      int q0, q_end, q1, seq_len, n, t;
-      sequence_shape(a, RB, s0 + lane, q0, q_end, q1, seq_len, n, t);
-      const int parts = max(1, (t + per - 1) / per), c = n * parts;
+      const SeqShape x = s0 == 0 ? own : sequence_shape(a, RB, s0 + lane);
+      const int parts = max(1, (x.t + per - 1) / per), c = x.n * parts;
       int incl = c;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int up = __shfl_up_sync(0xffffffffu, incl, o);
         if (lane >= o) incl += up;
       }
-      const int x = rowblk - acc;
-      const unsigned m = __ballot_sync(0xffffffffu, x < incl);
+      const int mine = rowblk - acc;
+      const unsigned m = __ballot_sync(0xffffffffu, mine < incl);
       if (m) {
         const int w = __ffs(m) - 1;
-        const int at = x - (incl - c), b = at / parts;  // (lane w: its block)
+        const int at = mine - (incl - c), b = at / parts;  // (lane w: its block)
         found = s0 + w;
-        first = __shfl_sync(0xffffffffu, q0 + b * RB, w);
-        nrows = __shfl_sync(0xffffffffu, min(RB, q1 - (q0 + b * RB)), w);
+        first = __shfl_sync(0xffffffffu, x.q0 + b * RB, w);
+        nrows = __shfl_sync(0xffffffffu, min(RB, x.q1 - (x.q0 + b * RB)), w);
         if (lane == w) {
-          s_info[3] = q_end;
-          s_info[4] = seq_len;
-          s_info[5] = q0;
+          s_info[3] = x.q_end;
+          s_info[4] = x.seq_len;
+          s_info[5] = x.q0;
           s_info[6] = at - b * parts;
           s_info[7] = parts;
         }
@@ -192,10 +206,26 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
       s_bad = 0;
     }
   }
-  if (warp == 1) {
+  // byte -> half2 tables (centroid[hi nibble], centroid[lo nibble]) scaled onto the fp16 grid: one with a copy a lane, or, for two codebooks,
+  // two with a copy for two lanes each
+  auto build_tables = [&](int t) {
+    bool one = true;
+    for (int i = 0; i < 16; ++i) one = one && s_cent[0][i] == s_cent[1][i];
+    uint4* lut = reinterpret_cast<uint4*>(sm + C::kOffLut);
+#pragma unroll 4
+    for (int i = t; i < (int)(C::kLut / 16); i += kDeq) {
+      const int e = one ? i / 8 : i / 4, w = e >> 8, b = e & 255;
+      const uint32_t v = pack_h2(s_cent[w][b >> 4], s_cent[w][b & 15]);
+      lut[i] = make_uint4(v, v, v, v);
+    }
+  };
+  if (warp >= kSmx / 32 && warp < kIssueWarp) {
+    // (every warp of them makes the same entries of s_cent)
     const int w = lane >> 4, i = lane & 15;
     const float* cent = w ? a.v_centroids : a.k_centroids;
     s_cent[w][i] = i < (w ? a.n_v_centroids : a.n_k_centroids) ? __fmul_rn(w ? a.lut_scale_v : a.lut_scale_k, __ldg(cent + i)) : 0.f;
+    __syncwarp();
+    if (FAST) build_tables(tid - kSmx);
   }
   __syncthreads();
   const int seq = s_info[0], row0 = s_info[1], nrows = s_info[2];
@@ -331,15 +361,10 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
     // ================= issuing thread =================
     if (n_tiles > 0 && elect_one_sync()) {
       bool ok = true;
-      uint32_t img_n = 0, img_ph = 0;  // images asked for / waited for
-      const bool unrotate = !pa.to_parts && !a.out_rotated;
-      const uint32_t ihi = base + C::kOffK, ilo = base + C::kOffLut;
-      auto load_image = [&]() {
-        ++img_n;
-        expect_tx(bar(s_bars.img), 2 * C::kImgTerm);
-        bulk_load(ihi, pa.image, C::kImgTerm, bar(s_bars.img));
-        bulk_load(ilo, pa.image + C::kImgTerm, C::kImgTerm, bar(s_bars.img));
-      };
+      uint32_t img_n = 0, img_ph = 0;  // phases of Pi's image asked for / waited for
+      const bool unrotate = !a.out_rotated;
+      constexpr uint32_t kTerms = FAST ? 1 : 2;
+      auto load_term = [&](int term, uint32_t to) { bulk_load(base + to, pa.image + term * C::kImgTerm, C::kImgTerm, bar(s_bars.img)); };
       // O = A * B: A = fp16 hi (and lo) terms at the S and Q columns, B = the image
       auto rotate = [&](bool unrot, bool a_lo) {
         ok = ok && bar_wait_own(bar(s_bars.img), img_ph & 1, dead);
@@ -348,18 +373,21 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
         if (!ok) return;
         fence_after();
         constexpr uint32_t d = C::kColO;
-        const uint32_t idesc = C::idesc(D, unrot);
+        const uint32_t idesc = C::idesc(D, unrot), ihi = base + (unrot ? C::kOffLut : C::kOffK), ilo = base + (unrot ? C::kOffK : C::kOffLut);
 #pragma unroll 1
         for (int s = 0; s < D / 16; ++s) {
           const uint32_t off = unrot ? 2048u * s : (s >> 2) * C::kImgPart + 32u * (s & 3);
           const uint64_t bh = make_desc(ihi + off, unrot ? C::kImgPart : 0), bl = make_desc(ilo + off, unrot ? C::kImgPart : 0);
-          mma_ta(tmem + d, tmem + C::kColS + 8 * s, bl, idesc, s > 0);
-          if (a_lo) mma_ta(tmem + d, tmem + C::kColQ + 8 * s, bh, idesc, true);
-          mma_ta(tmem + d, tmem + C::kColS + 8 * s, bh, idesc, true);
+          if (!FAST) mma_ta(tmem + d, tmem + C::kColS + 8 * s, bl, idesc, s > 0);
+          if (a_lo) mma_ta(tmem + d, tmem + C::kColQ + 8 * s, bh, idesc, !FAST || s > 0);
+          mma_ta(tmem + d, tmem + C::kColS + 8 * s, bh, idesc, !FAST || a_lo || s > 0);
         }
         mma_commit(bar(s_bars.rot));
       };
-      load_image();
+      ++img_n;
+      expect_tx(bar(s_bars.img), kTerms * C::kImgTerm);
+      load_term(0, C::kOffK);
+      if (!FAST) load_term(1, C::kOffLut);
       rotate(false, a.q_dtype == TQ4_F32);
 
       const uint64_t d_k = make_desc(base + C::kOffK, 0), d_v = make_desc(base + C::kOffV, kBN * 128);
@@ -393,7 +421,13 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
         issue_s();
       }
       for (int j = 0; j < n_tiles && ok; ++j) {
-        ok = bar_wait(bar(s_bars.vready[j % C::NVB]), (uint32_t)((j / C::NVB) & 1), dead) && bar_wait(bar(s_bars.pready), (uint32_t)(j & 1), dead);
+        ok = bar_wait(bar(s_bars.vready[j % C::NVB]), (uint32_t)((j / C::NVB) & 1), dead);
+        if (ok && j == n_tiles - 1 && unrotate) {  // (the tables have been read)
+          ++img_n;
+          expect_tx(bar(s_bars.img), kTerms * C::kImgTerm);
+          load_term(0, C::kOffLut);
+        }
+        ok = ok && bar_wait(bar(s_bars.pready), (uint32_t)(j & 1), dead);
         if (!ok) break;
         fence_after();
         issue_pv(j);
@@ -407,14 +441,17 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
       if (ok) {
         mma_commit(bar(s_bars.odone));
         ok = bar_wait_own(bar(s_bars.odone), 0u, dead);
-        if (ok && unrotate) {  // K~, V~ and the tables have been read
-          load_image();
+        if (ok && unrotate) {
+          if (!FAST) load_term(1, C::kOffK);  // (K~ and V~ have been read)
           rotate(true, true);
           if (ok) bar_wait_own(bar(s_bars.rot), 1u, dead);
         }
       }
       if (!ok) {  // (the CTA is dead)
-        if (img_n != img_ph) bar_wait_own(bar(s_bars.img), img_ph & 1, dead);
+        if (img_n != img_ph) {
+          if (!FAST && img_n == 2) load_term(1, C::kOffLut);  // (the phase is one of two terms; the place does not matter any more)
+          bar_wait_own(bar(s_bars.img), img_ph & 1, dead);
+        }
         mma_commit(bar(s_bars.drain));
         bar_wait_own(bar(s_bars.drain), 0u, dead);
       }
@@ -439,21 +476,13 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
       seg = C::NS - 1;
       return (C::NS & 1) && tok < kBN;
     };
-    bool ok = n_tiles > 0 && bar_wait(bar(s_bars.rot), 0u, dead);  // the image of Pi has been used: tables in place of its lo term
+    bool ok = n_tiles > 0 && bar_wait(bar(s_bars.rot), 0u, dead);  // the image of Pi has been used
     bool one_table = true;
     for (int i = 0; i < 16; ++i) one_table = one_table && s_cent[0][i] == s_cent[1][i];
-    // byte -> half2 tables (centroid[hi nibble], centroid[lo nibble]) scaled onto the fp16 grid: one with a copy a lane, or, for two codebooks,
-    // two with a copy for two lanes each
-    if (ok) {
-      uint4* lut = reinterpret_cast<uint4*>(sm + C::kOffLut);
-#pragma unroll 4
-      for (int i = t; i < (int)(C::kLut / 16); i += kDeq) {
-        const int e = one_table ? i / 8 : i / 4, w = e >> 8, b = e & 255;
-        const uint32_t v = pack_h2(s_cent[w][b >> 4], s_cent[w][b & 15]);
-        lut[i] = make_uint4(v, v, v, v);
-      }
+    if (!FAST) {  // tables in place of its lo term
+      if (ok) build_tables(t);
+      asm volatile("bar.sync 1, %0;" ::"n"(kDeq) : "memory");
     }
-    asm volatile("bar.sync 1, %0;" ::"n"(kDeq) : "memory");
     const uint32_t entry = one_table ? 128 : 64;  // bytes of a byte's copies
     const uint32_t lut_k = base + C::kOffLut + (lane & (entry / 4 - 1)) * 4, lut_v = lut_k + (one_table ? 0u : 256 * entry);
     auto look = [&](uint32_t at) -> uint32_t {
@@ -547,26 +576,55 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
         const bool q_vec = ((uintptr_t)a.q % 16 == 0) && (a.q_token_stride * es) % 16 == 0 && (a.q_head_stride * es) % 16 == 0;
         const int64_t qi = (int64_t)row * a.q_token_stride + (int64_t)head * a.q_head_stride;
         float sc = 1.f, isc = 1.f, amax = 0.f;
-#pragma unroll 1
-        for (int pass = 0; pass < 2; ++pass) {
-#pragma unroll 1
+        if (q_vec && es == 2) {  // all of a row's loads at once; the bits without the sign are in the order of the magnitudes
+          const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.q) + qi);
+          const bool f16 = a.q_dtype == TQ4_F16;
+          uint4 r[D / 8];
+#pragma unroll
+          for (int i = 0; i < D / 8; ++i) r[i] = live ? __ldg(src + i) : make_uint4(0u, 0u, 0u, 0u);
+          uint32_t top = 0;
+#pragma unroll
+          for (int i = 0; i < D / 8; ++i)
+            top = __vmaxu2(__vmaxu2(top, r[i].x & 0x7FFF7FFFu), __vmaxu2(r[i].y & 0x7FFF7FFFu, __vmaxu2(r[i].z & 0x7FFF7FFFu, r[i].w & 0x7FFF7FFFu)));
+          float x0, x1;
+          half_pair(top, f16, x0, x1);
+          pow2_scale(fmaxf(x0, x1), sc, isc);
+#pragma unroll
           for (int c = 0; c < D / 32; ++c) {
-            float x[32];
+            uint32_t h[16];
 #pragma unroll
-            for (int e = 0; e < 32; ++e) x[e] = 0.f;
-            if (live) load32(a.q, a.q_dtype, qi + 32 * c, q_vec, x);
-            if (pass == 0) {
+            for (int e = 0; e < 4; ++e) {
+              const uint32_t w[4] = {r[4 * c + e].x, r[4 * c + e].y, r[4 * c + e].z, r[4 * c + e].w};
 #pragma unroll
-              for (int e = 0; e < 16; ++e) amax = max3(amax, fabsf(x[2 * e]), fabsf(x[2 * e + 1]));
-            } else {
-              uint32_t h[16], l[16];
-#pragma unroll
-              for (int e = 0; e < 16; ++e) split2(x[2 * e] * sc, x[2 * e + 1] * sc, h[e], l[e]);
-              tmem_st16(tb + C::kColS + 16 * c, h);
-              if (a.q_dtype == TQ4_F32) tmem_st16(tb + C::kColQ + 16 * c, l);
+              for (int k = 0; k < 4; ++k) {
+                half_pair(w[k], f16, x0, x1);
+                h[4 * e + k] = pack_h2(x0 * sc, x1 * sc);
+              }
             }
+            tmem_st16(tb + C::kColS + 16 * c, h);
           }
-          if (pass == 0) pow2_scale(amax, sc, isc);
+        } else {
+#pragma unroll 1
+          for (int pass = 0; pass < 2; ++pass) {
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+              float x[32];
+#pragma unroll
+              for (int e = 0; e < 32; ++e) x[e] = 0.f;
+              if (live) load32(a.q, a.q_dtype, qi + 32 * c, q_vec, x);
+              if (pass == 0) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) amax = max3(amax, fabsf(x[2 * e]), fabsf(x[2 * e + 1]));
+              } else {
+                uint32_t h[16], l[16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) split2(x[2 * e] * sc, x[2 * e + 1] * sc, h[e], l[e]);
+                tmem_st16(tb + C::kColS + 16 * c, h);
+                if (a.q_dtype == TQ4_F32) tmem_st16(tb + C::kColQ + 16 * c, l);
+              }
+            }
+            if (pass == 0) pow2_scale(amax, sc, isc);
+          }
         }
         tmem_st_wait();
         arrive(s_bars.aready);
@@ -782,27 +840,8 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             *reinterpret_cast<uint4*>(reinterpret_cast<unsigned char*>(out) + at * elem + 16 * pc) = *reinterpret_cast<const uint4*>(rows + r * pitch + 16 * pc);
         }
       };
-      if (pa.to_parts || a.out_rotated) {
-        const int64_t vec = ((int64_t)s_info[6] * sh.rows + row) * sh.Hq + head;
-#pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
-          uint32_t v[32];
-          if (use && ok) tmem_ld32(tb + C::kColO + 32 * c, v);
-          float y[32];
-#pragma unroll
-          for (int e = 0; e < 32; ++e) y[e] = have ? __uint_as_float(v[e]) * inv : 0.f;
-          if (pa.to_parts) {
-            float4* dst = reinterpret_cast<float4*>(sm + (uint32_t)m * C::kPartPitch + 128 * c);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) dst[e] = make_float4(y[4 * e], y[4 * e + 1], y[4 * e + 2], y[4 * e + 3]);
-          } else if (live) {
-            store32(a.out, a.out_dtype, oi + 32 * c, out_vec, y);
-          }
-        }
-        if (pa.to_parts) store_rows(C::kPartPitch, 4 * D, pa.part_o, 4, live && have ? vec * D : -1);  // (an empty partial's sums are not read)
-        if (live && pa.to_parts) pa.part_m[vec] = lse;
-        else if (live && a.lse_out) a.lse_out[(int64_t)row * sh.Hq + head] = lse;
-      } else {
+      float f = inv;
+      if (!a.out_rotated) {  // (parts, too: the merge is linear)
         float isc = 0.f;
         if (use) {
           float amax = 0.f, sc = 1.f;
@@ -831,23 +870,33 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
           ok = __all_sync(0xffffffffu, bar_wait(bar(s_bars.rot), 1u, dead)) && ok;
           fence_after();
         }
-        const float f = have && ok ? isc * (1.f / 256.f) : 0.f;
-        const bool staged = out_vec && a.out_dtype != TQ4_F32;
+        f = have && ok ? isc * (1.f / 256.f) : 0.f;
+      }
+      const int64_t vec = ((int64_t)s_info[6] * sh.rows + row) * sh.Hq + head;
+      const bool staged = pa.to_parts || (out_vec && a.out_dtype != TQ4_F32);
 #pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
-          uint32_t v[32];
-          if (use && ok) tmem_ld32(tb + C::kColO + 32 * c, v);
-          if (live) {
-            float y[32];
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t v[32];
+        if (use && ok) tmem_ld32(tb + C::kColO + 32 * c, v);
+        if (live) {
+          float y[32];
 #pragma unroll
-            for (int e = 0; e < 32; ++e) y[e] = f != 0.f ? __uint_as_float(v[e]) * f : 0.f;
-            if (staged) store32(sm + (uint32_t)m * C::kOutPitch, a.out_dtype, 32 * c, true, y);
-            else store32(a.out, a.out_dtype, oi + 32 * c, out_vec, y);
+          for (int e = 0; e < 32; ++e) y[e] = f != 0.f ? __uint_as_float(v[e]) * f : 0.f;
+          if (pa.to_parts) {
+            float4* dst = reinterpret_cast<float4*>(sm + (uint32_t)m * C::kPartPitch + 128 * c);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) dst[e] = make_float4(y[4 * e], y[4 * e + 1], y[4 * e + 2], y[4 * e + 3]);
+          } else if (staged) {
+            store32(sm + (uint32_t)m * C::kOutPitch, a.out_dtype, 32 * c, true, y);
+          } else {
+            store32(a.out, a.out_dtype, oi + 32 * c, out_vec, y);
           }
         }
-        if (staged) store_rows(C::kOutPitch, 2 * D, a.out, 2, live ? oi : -1);
-        if (live && a.lse_out) a.lse_out[(int64_t)row * sh.Hq + head] = lse;
       }
+      if (pa.to_parts) store_rows(C::kPartPitch, 4 * D, pa.part_o, 4, live && have ? vec * D : -1);  // (an empty partial's sums are not read)
+      else if (staged) store_rows(C::kOutPitch, 2 * D, a.out, 2, live ? oi : -1);
+      if (live && pa.to_parts) pa.part_m[vec] = lse;
+      else if (live && a.lse_out) a.lse_out[(int64_t)row * sh.Hq + head] = lse;
     }
   }
   fence_before();
