@@ -391,8 +391,9 @@ int tq4_tree_mask(const int32_t* parents, const int32_t* query_start_loc, int64_
  * of its set bits, minus 1, and of the former it sees those within the window; the drafts are the mask's alone.
  * tree_mask int32 [num_rows, tree_mask_words] and block_table int32 [num_seqs, bt_width] with row strides in elements; a sequence
  * longer than its row of the table is cut there (TQ4_DEV_BAD_BLOCK).  max_seq_len as in tq4_attention_step; the other arguments,
- * checks and the precision are those of tq4_paged_attention in the prefill form, with at most 128 query heads per KV head.  A row that
- * sees no key, or past the last offset, gets zeros and an lse of -inf.
+ * checks and the precision are those of tq4_paged_attention in the prefill form, with at most 128 query heads per KV head; but a call
+ * with bf16 queries, a bf16 output and no lse_out may round rotated queries and weights to fp16 (4e-4 of relative 2-norm, beside the
+ * output's own 1.7e-3).  A row that sees no key, or past the last offset, gets zeros and an lse of -inf.
  * workspace >= tq4_tree_attention_workspace_bytes(num_rows, Hq, Hkv, D), 16-byte aligned.
  */
 size_t tq4_tree_attention_workspace_bytes(int64_t max_query_rows, int num_q_heads, int num_kv_heads, int head_dim);
@@ -418,7 +419,7 @@ int tq4_tree_attention(const void* q, int q_dtype, int64_t num_rows, int num_seq
  * int64 [n_pairs, 2] on the device.  A page may be the destination of one pair only and not also a source (other than of itself,
  * which does nothing): of several pairs with one destination the first counts, and a pair whose source is another's destination
  * is not carried out; both raise TQ4_DEV_PAGE_CONFLICT, unless the pairs are equal.  A page out of range raises TQ4_DEV_BAD_BLOCK.
- * workspace: tq4_copy_blocks_workspace_bytes (0 for up to 1024 pairs: may be null).
+ * workspace: tq4_copy_blocks_workspace_bytes (0 for up to 384 pairs: may be null).
  */
 size_t tq4_copy_blocks_workspace_bytes(int64_t n_pairs, int64_t num_blocks);
 int tq4_copy_blocks(uint8_t* const* caches, int num_caches, int64_t num_blocks, int block_size, int64_t cache_block_stride,

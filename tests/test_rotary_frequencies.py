@@ -98,7 +98,7 @@ def test_status_of_the_c_entry_points_without_a_launch(cuda_lib):
     assert lib.tq4_copy_blocks(at, 1, 8, 16, 16 * 272, 272, 2, 128, None, 1, 3, None, 0, None, None) == invalid
     assert lib.tq4_copy_blocks(at, 1, 8, 16, 16 * 272, 271, 2, 128, at, 1, 3, None, 0, None, None) == invalid
     assert lib.tq4_copy_blocks(at, 1, 8, 16, 16 * 272, 272, 2, 100, at, 1, 3, None, 0, None, None) == unsupported
-    assert lib.tq4_copy_blocks_workspace_bytes(1024, 50) == 0 and lib.tq4_copy_blocks_workspace_bytes(1025, 50) == 200
+    assert lib.tq4_copy_blocks_workspace_bytes(384, 50) == 0 and lib.tq4_copy_blocks_workspace_bytes(385, 50) == 200
     assert lib.tq4_copy_blocks(at, 1, 8, 16, 16 * 272, 272, 2, 128, at, 1, 1025, None, 0, None, None) == workspace
     assert lib.tq4_compact_rows_workspace_bytes(3, 2, 64, 2, 128) == 0
     need = lib.tq4_compact_rows_workspace_bytes(3, 2, 65, 2, 128)

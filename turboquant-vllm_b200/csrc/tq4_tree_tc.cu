@@ -15,8 +15,9 @@
 // Roles: warps 0 - 3 softmax (a thread a row), 4 - 7 dequantisation, 8 the issuing thread, 9 the fetching lanes.  They meet at
 // mbarriers; every wait is bounded as in the prefill kernel.
 //
-// FAST: the terms of queries and probabilities that 11 bits leave out stay out, half the tensor work.  Used where the output is bf16, whose own
-// rounding is 2^-9 of a value: a rounding of 2^-12 of queries and weights moves it by 5e-4 of its norm, against 1.7e-3.
+// FAST: the terms of queries and probabilities that 11 bits leave out stay out, half the tensor work.  Used where queries and output are
+// bf16 and no lse is asked for: the queries have lost 2^-9 of a coordinate and the output will, and a rounding of 2^-12 of queries
+// and weights moves it by 4e-4 of its norm, beside 1.7e-3 of its own.  (An fp16 output's rounding is 2e-4: both terms stay.)
 #include <math_constants.h>
 
 #include <cstdlib>
@@ -388,7 +389,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
       expect_tx(bar(s_bars.img), kTerms * C::kImgTerm);
       load_term(0, C::kOffK);
       if (!FAST) load_term(1, C::kOffLut);
-      rotate(false, a.q_dtype == TQ4_F32);
+      rotate(false, !FAST && a.q_dtype == TQ4_F32);
 
       const uint64_t d_k = make_desc(base + C::kOffK, 0), d_v = make_desc(base + C::kOffV, kBN * 128);
       const uint64_t d_qlo = make_desc(base + C::kOffQlo, 0);
@@ -969,7 +970,7 @@ int launch_tree_few(const AttnArgs& a, cudaStream_t st, int splits, bool to_part
   const TreeArgs pa{image, splits, tree_few_slots(a), to_parts ? 1 : 0, part_o, part_m};
   const int rc = launch_pi_image(a.sh.D, a.rotation, image, st);
   if (rc != TQ4_OK) return rc;
-  const bool fast = a.out_dtype == TQ4_BF16;
+  const bool fast = a.q_dtype == TQ4_BF16 && a.out_dtype == TQ4_BF16 && a.lse_out == nullptr;
   switch (a.sh.D) {
     case 64: return fast ? launch_t<64, true>(a, pa, st) : launch_t<64, false>(a, pa, st);
     case 96: return fast ? launch_t<96, true>(a, pa, st) : launch_t<96, false>(a, pa, st);

@@ -555,7 +555,8 @@ def paged_tq4_tree_attention(
     drafts those whose bits are set in its row of ``tree_mask`` (:func:`tq4_tree_mask`, or any other int32 ``[T, words]``).
     ``sliding_window``: of the keys in front of the drafts, those within the window of the row's position, which is that of the last
     of them plus the number of its set bits; the drafts are left to the mask.  A row that sees nothing gets zeros (``lse_out``: -inf).
-    The other arguments, and the precision, are those of :func:`paged_tq4_attention`.
+    The other arguments, and the precision, are those of :func:`paged_tq4_attention`; but bf16 queries with a bf16 output and no
+    ``lse_out`` may enter the tensor cores as single fp16 terms, as the weights (4e-4 of the output's norm, beside 1.7e-3 that bf16 costs).
     """
     return nv.host().tree_attention(
         q, kv_cache, block_table, seq_lens, query_start_loc, tree_mask, k_centroids, v_centroids, rotation, num_kv_heads, block_size,
