@@ -217,8 +217,8 @@ int tree_tc_splits(const AttnArgs& a, int64_t slots);
 int launch_pi_image(int D, const float* rotation, uint8_t* image, cudaStream_t st);
 bool tree_few_supported(const AttnArgs& a);
 int tree_few_splits(const AttnArgs& a, int64_t room);
-int launch_tree_few(const AttnArgs& a, cudaStream_t st, int splits, bool to_parts, uint8_t* image, float* part_o, float* part_m);
-int launch_tree_tc(const AttnArgs& a, cudaStream_t st, int splits, bool to_parts, uint8_t* image, float* part_o, float* part_m);
+int launch_tree_few(const AttnArgs& a, cudaStream_t st, bool fast, int splits, bool to_parts, uint8_t* image, float* part_o, float* part_m);
+int launch_tree_tc(const AttnArgs& a, cudaStream_t st, bool fast, int splits, bool to_parts, uint8_t* image, float* part_o, float* part_m);
 constexpr int kPrefillMinRows = 8;  // new rows of a sequence from which the prefill kernel is the faster one
 int mma_warps_per_cta(int D, int GC, int Hkv, int64_t token_stride = 0);
 bool attention_mma_supported(const AttnShape& sh, int block_size, const uint8_t* cache,

@@ -1208,8 +1208,7 @@ int launch_d(const AttnArgs& a, const PrefillArgs& pa, cudaStream_t st, bool fas
   // first kernel of the prefill part: a plain launch (what the caller and the streaming part wrote is complete)
   const int rc = launch_image<D>(a.rotation, image, st);
   if (rc != TQ4_OK) return rc;
-  if constexpr (!TREE)
-    if (fast) return launch_t<D, true, false>(a, pa, st);
+  if (fast) return launch_t<D, true, TREE>(a, pa, st);
   return launch_t<D, false, TREE>(a, pa, st);
 }
 
@@ -1272,13 +1271,13 @@ int tree_tc_splits(const AttnArgs& a, int64_t slots) {
   return s < 1 ? 1 : (int)s;
 }
 
-int launch_tree_tc(const AttnArgs& a, cudaStream_t st, int splits, bool to_parts, uint8_t* image, float* part_o, float* part_m) {
+int launch_tree_tc(const AttnArgs& a, cudaStream_t st, bool fast, int splits, bool to_parts, uint8_t* image, float* part_o, float* part_m) {
   const PrefillArgs pa{image, 1, splits, to_parts ? 1 : 0, part_o, part_m};
   switch (a.sh.D) {
-    case 64: return launch_d<64, true>(a, pa, st, false, image);
-    case 96: return launch_d<96, true>(a, pa, st, false, image);
-    case 128: return launch_d<128, true>(a, pa, st, false, image);
-    case 256: return launch_d<256, true>(a, pa, st, false, image);
+    case 64: return launch_d<64, true>(a, pa, st, fast, image);
+    case 96: return launch_d<96, true>(a, pa, st, fast, image);
+    case 128: return launch_d<128, true>(a, pa, st, fast, image);
+    case 256: return launch_d<256, true>(a, pa, st, fast, image);
   }
   return TQ4_ERR_UNSUPPORTED;
 }

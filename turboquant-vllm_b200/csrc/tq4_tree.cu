@@ -175,15 +175,18 @@ extern "C" int tq4_tree_attention(
   float* part_o = reinterpret_cast<float*>(image + prefill_tc_image_bytes(head_dim));
   const int64_t room = (int64_t)((uintptr_t)workspace + workspace_bytes) - (int64_t)(uintptr_t)part_o;
   // The kernel for few drafts takes 128 / G rows of a sequence a CTA, the other twice that: the first, unless sequences fill more than one of
-  // its CTAs on average, which would dequantise every tile again.
+  // its CTAs on average, which would dequantise every tile again.  64 sequences of 4096 tokens, 32 / 8 heads of 128, bf16, few / other:
+  // 32 drafts (128 rows) 265 / 421 us, 64 drafts 518 / 509, 128 drafts 984 / 912 (fp16: 339 / 451, 662 / 616, 1261 / 1079).
   const bool few = tree_few_supported(a) && num_rows * a.sh.G <= 128 * (int64_t)(num_seqs > 0 ? num_seqs : 1);
+  // queries and weights as single fp16 terms: half the products, where bf16 has lost more of the queries and will lose more of the output
+  const bool fast = a.q_dtype == TQ4_BF16 && out_dtype == TQ4_BF16 && !lse_out;
   const int64_t slots = room / ((int64_t)num_q_heads * (head_dim + 1) * 4) - 1;
   const int splits = few ? tree_few_splits(a, slots) : tree_tc_splits(a, slots);
   const bool to_parts = splits > 1;
   float* part_m = part_o + (size_t)splits * num_rows * num_q_heads * head_dim;
   prof_begin(TQ4_PROF_ATTENTION, st);
-  const int rc = few ? launch_tree_few(a, st, splits, to_parts, image, part_o, part_m)
-                     : launch_tree_tc(a, st, splits, to_parts, image, part_o, part_m);
+  const int rc = few ? launch_tree_few(a, st, fast, splits, to_parts, image, part_o, part_m)
+                     : launch_tree_tc(a, st, fast, splits, to_parts, image, part_o, part_m);
   prof_end(TQ4_PROF_ATTENTION, st);
   if (rc != TQ4_OK || !to_parts) return rc;
   CombineArgs c{};

@@ -966,11 +966,10 @@ int tree_few_splits(const AttnArgs& a, int64_t room) {
   return s < 1 ? 1 : (int)s;
 }
 
-int launch_tree_few(const AttnArgs& a, cudaStream_t st, int splits, bool to_parts, uint8_t* image, float* part_o, float* part_m) {
+int launch_tree_few(const AttnArgs& a, cudaStream_t st, bool fast, int splits, bool to_parts, uint8_t* image, float* part_o, float* part_m) {
   const TreeArgs pa{image, splits, tree_few_slots(a), to_parts ? 1 : 0, part_o, part_m};
   const int rc = launch_pi_image(a.sh.D, a.rotation, image, st);
   if (rc != TQ4_OK) return rc;
-  const bool fast = a.q_dtype == TQ4_BF16 && a.out_dtype == TQ4_BF16 && a.lse_out == nullptr;
   switch (a.sh.D) {
     case 64: return fast ? launch_t<64, true>(a, pa, st) : launch_t<64, false>(a, pa, st);
     case 96: return fast ? launch_t<96, true>(a, pa, st) : launch_t<96, false>(a, pa, st);
