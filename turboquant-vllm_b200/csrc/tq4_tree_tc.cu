@@ -114,7 +114,8 @@ __device__ __forceinline__ SeqShape sequence_shape(const AttnArgs& a, int RB, in
 // The fewest tiles a key part with which all parts of a KV head find a slot at once (a warp; `x`: the lane's sequence of the first 32; out of
 // the way of the code that is run often).
 __device__ __noinline__ int tiles_per_part(const AttnArgs& a, const TreeArgs& pa, int RB, int lane, int n0, int t0) {
-  int longest = 0;
+  int longest = 0, blocks = 0;
+  long long tiles = 0;
   for (int s0 = 0; s0 < a.sh.num_seqs; s0 += 32) {
     int n = n0, t = t0;
     if (s0 > 0) {
@@ -123,8 +124,14 @@ __device__ __noinline__ int tiles_per_part(const AttnArgs& a, const TreeArgs& pa
       t = x.t;
     }
     longest = max(longest, __reduce_max_sync(0xffffffffu, n > 0 ? t : 0));
+    blocks += __reduce_add_sync(0xffffffffu, n);
+    const long long x = (long long)n * t;  // (in two sums of 32 lanes that 32 bits hold)
+    tiles += ((long long)__reduce_add_sync(0xffffffffu, (unsigned)(x >> 20)) << 20) + __reduce_add_sync(0xffffffffu, (unsigned)x & 0xFFFFFu);
   }
+  // (the parts of n blocks of t tiles are n t / per at least, and n more than that at most)
   int lo = max(kMinTiles, (longest + pa.splits - 1) / pa.splits), hi = max(lo, longest);
+  lo = max(lo, (int)min((long long)hi, (tiles + pa.slots - 1) / pa.slots));
+  if (blocks < pa.slots) hi = max(lo, (int)min((long long)hi, tiles / (pa.slots - blocks) + 1));
   while (lo < hi) {
     const int mid = (lo + hi) / 2;
     int parts = 0;
@@ -579,7 +586,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
         float sc = 1.f, isc = 1.f, amax = 0.f;
         if (q_vec && es == 2) {  // all of a row's loads at once; the bits without the sign are in the order of the magnitudes
           const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.q) + qi);
-          const bool f16 = a.q_dtype == TQ4_F16;
+          const bool f16 = !FAST && a.q_dtype == TQ4_F16;  // (FAST: bf16)
           uint4 r[D / 8];
 #pragma unroll
           for (int i = 0; i < D / 8; ++i) r[i] = live ? __ldg(src + i) : make_uint4(0u, 0u, 0u, 0u);
