@@ -393,7 +393,8 @@ int tq4_tree_mask(const int32_t* parents, const int32_t* query_start_loc, int64_
  * longer than its row of the table is cut there (TQ4_DEV_BAD_BLOCK).  max_seq_len as in tq4_attention_step; the other arguments,
  * checks and the precision are those of tq4_paged_attention in the prefill form, with at most 128 query heads per KV head; but a call
  * with bf16 queries, a bf16 output and no lse_out may round rotated queries and weights to fp16 (4e-4 of relative 2-norm, beside the
- * output's own 1.7e-3).  A row that sees no key, or past the last offset, gets zeros and an lse of -inf.
+ * output's own 1.7e-3).  A row that sees no key, or past the last offset, gets zeros and an lse of -inf.  An
+ * infinite or NaN norm in the cache makes the rows that see its token NaN, and no others.
  * workspace >= tq4_tree_attention_workspace_bytes(num_rows, Hq, Hkv, D), 16-byte aligned.
  */
 size_t tq4_tree_attention_workspace_bytes(int64_t max_query_rows, int num_q_heads, int num_kv_heads, int head_dim);

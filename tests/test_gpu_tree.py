@@ -384,3 +384,37 @@ def test_captured_calls_on_two_streams_and_an_own_workspace(ops):
         torch.cuda.synchronize()
         for _, out, eager, *_ in cases:
             assert torch.equal(out, eager)
+
+
+@pytest.mark.parametrize("lens,nodes", [([100], [20]), ([3000, 70], [30, 3]), ([400], [200])])  # one part, parts of the keys, many drafts
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("where", ["key", "value"])
+@pytest.mark.parametrize("bad", [math.inf, math.nan])
+def test_a_norm_that_is_not_finite_reaches_the_rows_that_see_it(ops, lens, nodes, dtype, where, bad):
+    """In a draft, and in front of the window: rows that do not see the token are what they were, the others NaN."""
+    d, hkv, bs, window = 128, 2, 16, 40
+    pr = Prims(d)
+    p = pr.cuda()
+    case = build_paged_case(lens, hkv, d, bs, pr, seed=6, padded=True)
+    matrices = ancestor_matrix(nodes, random_parents(nodes, random.Random(2), 3))
+    mask = pack(matrices, -(-max(nodes) // 32))
+    q = torch.randn(sum(nodes), 8, d, generator=torch.Generator().manual_seed(3)).to(DTYPES[dtype])
+    for window_, token in ((None, lens[0] - nodes[0] + 4), (window, lens[0] - nodes[0] - window)):
+        good = _call(ops, q, case, nodes, mask, p, hkv, bs, sliding_window=window_)
+        assert torch.isfinite(good).all()
+        hurt = dict(case, cache=case["cache"].clone())
+        at = hkv * d // 2 if where == "key" else hkv * d + 4 * hkv
+        row = hurt["cache"][case["block_table"][0, token // bs].long(), token % bs]
+        row[at : at + 4] = torch.tensor([bad]).view(torch.uint8)  # (the first KV head's)
+        got = _call(ops, q, hurt, nodes, mask, p, hkv, bs, sliding_window=window_)
+        sees = torch.zeros(sum(nodes), dtype=torch.bool)
+        if window_ is None:
+            sees[: nodes[0]] = torch.from_numpy(matrices[0][:, 4])
+        else:  # (the position of a row of depth n - 1 is that of the last token held plus n)
+            sees[: nodes[0]] = torch.from_numpy(token >= lens[0] - nodes[0] + matrices[0].sum(axis=1) - window)
+        hit = torch.zeros(sum(nodes), 8, dtype=torch.bool)
+        hit[sees, :4] = True
+        assert 0 < int(sees.sum()) < sum(nodes) or window_ is not None
+        assert torch.isnan(got.cpu()[hit]).all()
+        assert torch.equal(got.cpu()[~hit], good.cpu()[~hit])
+    assert ops.read_and_clear_errors(q.cuda().device) == 0

@@ -647,6 +647,11 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(const AttnArgs 
             // (positive, so that -inf times it stays -inf)
             ns[tok] = it[n].kn == kHidden ? kHidden : fmaxf(it[n].kn, 1e-30f) * (1.f / kQGain);
             ns[kBN + tok] = it[n].vn;
+            if (TREE && !(fabsf(it[n].kn) < CUDART_INF_F && fabsf(it[n].vn) < CUDART_INF_F)) {  // (a weight of zero times it is none)
+              s_bad = 1;
+              ns[tok] = kNotFinite;
+              ns[kBN + tok] = 0.f;
+            }
           }
         }
       }
@@ -901,8 +906,10 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(const AttnArgs 
                 if (n > 0 && k > -32) vis[w] |= draft_bits(k) & (0xFFFFFFFFu >> (32 - n));
               }
               if (*(volatile int*)&s_bad)
-                for (int i = 0; i < 32; ++i)
+                for (int i = 0; i < 32; ++i) {
                   if (ns[32 * w + i] == kHidden) vis[w] &= ~(1u << i);
+                  if (TREE && ns[32 * w + i] == kNotFinite && (vis[w] >> i & 1u)) l_run = CUDART_NAN_F;
+                }
               seen = seen || vis[w];
             }
 #pragma unroll
@@ -1024,7 +1031,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(const AttnArgs 
     if (use) {
       ok = __all_sync(0xffffffffu, ok && bar_wait(bar(s_bars.odone), 0u, dead));
       fence_after();
-      have = ok && l_run > 0.f;
+      have = ok && (TREE ? l_run != 0.f : l_run > 0.f);
     }
     if (streams && n_blk == 2) {  // (uniform) the second stream's sums into the first's
       float* s_o = reinterpret_cast<float*>(sm + C::kOffK);  // [128][D] where K~ and V~ were, 16-byte pieces of a row rotated by it
@@ -1051,7 +1058,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(const AttnArgs 
         const float f0 = ex2_approx(m_run - ref), f1 = ex2_approx(other.x - ref);
         m_run = top;
         l_run = l_run * f0 + other.y * f1;
-        have = ok && l_run > 0.f;
+        have = ok && (TREE ? l_run != 0.f : l_run > 0.f);
 #pragma unroll 1
         for (int q = 0; q < DPT / 16; ++q) {
           uint32_t o[16];

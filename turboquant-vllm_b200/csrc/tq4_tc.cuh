@@ -8,6 +8,7 @@ namespace {
 
 constexpr int kBN = 64;         // tokens per tile
 constexpr float kHidden = 1e-33f;  // key norm in shared memory of a token whose page id is out of range
+constexpr float kNotFinite = 2e-33f;  // ... of one that has an infinite or NaN norm (trees): NaN to the rows that see it, nothing to others
 constexpr float kQGain = 64.f;     // factor of the queries' terms, its inverse in the key norms: keeps the lo terms normal numbers
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }

@@ -161,7 +161,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
   __shared__ uint32_t s_tmem;
   __shared__ int s_info[8];        // sequence, first row and rows of the CTA; end of the sequence's rows, its length, their start; key part, parts
   __shared__ float s_cent[2][16];  // scaled centroids of K and V
-  __shared__ int s_dead, s_bad;    // a wait gave up / some page id is out of range
+  __shared__ int s_dead, s_bad;    // a wait gave up / some page id is out of range, or some norm is not finite
   __shared__ int s_badgrp[2];      // groups of the stage's tile whose page id is
   const AttnShape& sh = a.sh;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -531,8 +531,10 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
         float kn = *reinterpret_cast<const float*>(raw + C::kRawKn + 16 * t + kn_off), vn = *reinterpret_cast<const float*>(raw + C::kRawVn + 16 * t + vn_off);
         const bool past = t_first + j * kBN + t >= len, bad = s_badgrp[st] >> (t / kGroup) & 1;
         // (positive, so that -inf times it stays -inf; what lies past the sequence is masked, whatever was there)
-        ns[t] = past ? 1.f : bad ? kHidden : fmaxf(kn, 1e-30f) * (1.f / kQGain);
-        ns[kBN + t] = past || bad ? 0.f : vn;
+        const bool odd = !past && !bad && !(fabsf(kn) < CUDART_INF_F && fabsf(vn) < CUDART_INF_F);  // (a weight of zero times it is none)
+        if (odd) s_bad = 1;
+        ns[t] = past ? 1.f : bad ? kHidden : odd ? kNotFinite : fmaxf(kn, 1e-30f) * (1.f / kQGain);
+        ns[kBN + t] = past || bad || odd ? 0.f : vn;
       }
 #pragma unroll
       for (int n = 0; n < NIT; ++n) {
@@ -716,8 +718,11 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
               if (n > 0 && k > -32) vis[w] |= draft_bits(k) & (0xFFFFFFFFu >> (32 - n));
             }
             if (any_bad)
-              for (int i = 0; i < 32; ++i)
-                if (ns[32 * w + i] == kHidden) vis[w] &= ~(1u << i);
+              for (int i = 0; i < 32; ++i) {
+                const float kn = ns[32 * w + i];
+                if (kn == kHidden) vis[w] &= ~(1u << i);
+                if (kn == kNotFinite && (vis[w] >> i & 1u)) l_run = CUDART_NAN_F;
+              }
             seen = seen || vis[w];
           }
 #pragma unroll
@@ -828,7 +833,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
       if (use) {
         ok = __all_sync(0xffffffffu, ok && bar_wait(bar(s_bars.odone), 0u, dead));
         fence_after();
-        have = ok && l_run > 0.f;
+        have = ok && l_run != 0.f;  // (NaN: handed on)
       }
       const float inv = have ? 1.f / (a.lut_scale_v * l_run) : 0.f;
       const float lse = have ? (m_run + lg2_approx(l_run)) * 0.6931471805599453f : -CUDART_INF_F;
