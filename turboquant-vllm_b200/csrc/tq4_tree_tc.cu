@@ -9,9 +9,18 @@
 // as long as all of these (a dequantising warp spent 1300 - 1900 of 2800 cycles a tile issuing them).  Hence:
 //   * the packed rows come by TMA boxes of 16 tokens, asked for by a warp of its own;
 //   * two CTAs share an SM, of 256 tensor-memory columns and half the shared memory each: one's set-up, softmax and
-//     rotations fill the other's waits.  Single K~ and V~ buffers are enough: keys are written during the softmax of the tile
-//     before, values during the scores and softmax of their own;
+//     rotations fill the other's waits.  One K~ buffer is enough: keys are written during the softmax of the tile before.  V~ has
+//     two where there is room (all but two-term head_dim 128), which is worth 3 %;
 //   * warps without a draft take no part.
+// Measured (graph replays; in brackets the floor by bytes or operations), us: 8 drafts behind 1024 tokens of 28 / 4 heads of 128 21.7 (0.1);
+// 16 sequences of 300 to 8100 tokens, 5 to 24 drafts, 32 / 8 heads, fp16 108 (11.8); 64 of 4096 with 16 drafts, bf16 230 (46); 8 of
+// 65536 with 48 to 64 drafts, 32 / 32 heads of 96 1480 (268).  A call of few tiles is its chain: 13 thousand cycles of search, queries and
+// rotation, 6 of the first tile, 8 of un-rotation and stores.  In long ones a CTA takes 3000 cycles a tile: keys 1200 and values 1000 of
+// the dequantising warps, and 750 for their four waits; the softmax warps need 1600 of them, the products 530.  The load/store pipe is
+// 56 % busy with wavefronts and some 17 % more with operand reads and boxes: items of the same warps take twice as long with two
+// CTAs as with one.  What took work off one of the groups moved it to the other, and none of it paid: rows of fewer than 64
+// twice or four times among the 128, each with its share of a tile's columns, softmax 770 cycles a tile, 247 us instead of 234 at 64 x 4096; the
+// norms by the softmax warps, 246; half of the values as well, 298; eight dequantising warps, 278; permutes for the values' table, 253.
 // Roles: warps 0 - 3 softmax (a thread a row), 4 - 7 dequantisation, 8 the issuing thread, 9 the fetching lanes.  They meet at
 // mbarriers; every wait is bounded as in the prefill kernel.
 //
@@ -174,7 +183,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
   // ---- which rows and keys are this CTA's? -----------------------------------------------------------------------
   // A sequence's rows make n blocks of RB rows, its keys t tiles; in a call cut along the keys every block has ceil(t / per) parts, with
   // the fewest tiles a part, `per`, for which all parts find a slot at once: long sequences are cut into more.  (As many parts for all of
-  // them: 16 of 300 to 8100 tokens 157 us, 115 so.)
+  // them: 16 of 300 to 8100 tokens 157 us where this took 115.)
   if (warp == 0) {
     const SeqShape own = sequence_shape(a, RB, lane);
     const int per = pa.to_parts ? tiles_per_part(a, pa, RB, lane, own.n, own.t) : 0x3fffffff;
