@@ -418,3 +418,66 @@ def test_a_norm_that_is_not_finite_reaches_the_rows_that_see_it(ops, lens, nodes
         assert torch.isnan(got.cpu()[hit]).all()
         assert torch.equal(got.cpu()[~hit], good.cpu()[~hit])
     assert ops.read_and_clear_errors(q.cuda().device) == 0
+
+
+def test_more_sequences_than_a_warp_has_lanes_cut_along_the_keys(ops):
+    """Seventy sequences of very different lengths, some empty, on one KV head: the shares of the keys are found 32 sequences at a time."""
+    rng = random.Random(7)
+    d, hq, hkv, bs = 128, 4, 1, 16
+    nodes = [rng.choice((0, 1, 5, 30)) for _ in range(70)]
+    lens = [n + rng.choice((0, 3, 64, 500, 1500)) for n in nodes]
+    pr = Prims(d)
+    case = build_paged_case(lens, hkv, d, bs, pr, seed=5, padded=True)
+    matrices = ancestor_matrix(nodes, random_parents(nodes, rng))
+    q = torch.randn(sum(nodes), hq, d, generator=torch.Generator().manual_seed(1)).half()
+    lse = torch.full((sum(nodes), hq), math.nan, device="cuda")
+    got = _call(ops, q, case, nodes, pack(matrices, 1), pr.cuda(), hkv, bs, out_dtype=torch.float32, lse_out=lse)
+    want, want_lse, spread = reference(q, case, nodes, matrices, pr, hkv, bs, d ** -0.5)
+    _check(got.cpu(), lse.cpu(), want, want_lse, spread)
+    assert ops.read_and_clear_errors(got.device) == 0
+
+
+@pytest.mark.parametrize("d,hq,hkv", [(128, 8, 2), (256, 8, 4)])
+def test_a_replayed_graph_follows_lengths_offsets_and_masks(ops, d, hq, hkv):
+    """The step that a server captures once: its inputs change in place, sequences come and go, the mask is part of a wider buffer."""
+    pr = Prims(d)
+    p = pr.cuda()
+    cases = [([900, 40, 0], [7, 20, 0]), ([5, 0, 1700], [5, 0, 31]), ([64, 2000, 33], [1, 2, 3])]
+    rows, words = 40, 2
+    built = [build_paged_case(lens, hkv, d, 16, pr, seed=i, padded=True) for i, (lens, _) in enumerate(cases)]
+    pages = max(b["cache"].shape[0] for b in built)
+    width = max(b["block_table"].shape[1] for b in built) + 3
+    cache = torch.zeros(pages, *built[0]["cache"].shape[1:], dtype=torch.uint8, device="cuda")
+    table = torch.zeros(3, width, dtype=torch.int32, device="cuda")
+    lens_, starts = torch.zeros(3, dtype=torch.int32, device="cuda"), torch.zeros(4, dtype=torch.int32, device="cuda")
+    mask = torch.full((rows, words + 3), -1, dtype=torch.int32, device="cuda")
+    q = torch.zeros(rows, hq, d, dtype=torch.bfloat16, device="cuda")
+    out, lse = torch.zeros(rows, hq, d, device="cuda"), torch.zeros(rows, hq, device="cuda")
+
+    def step():
+        ops.paged_tq4_tree_attention(q, cache, table, lens_, starts, mask[:, 1 : 1 + words], p["kc"], p["vc"], p["rot"], hkv, 16, out=out, lse_out=lse)
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for i in (0, 1, 2, 0):
+        (lens, nodes), case = cases[i], built[i]
+        n = sum(nodes)
+        matrices = ancestor_matrix(nodes, random_parents(nodes, random.Random(i)))
+        cache[: case["cache"].shape[0]].copy_(case["cache"])
+        table.zero_()
+        table[:, : case["block_table"].shape[1]].copy_(case["block_table"])
+        lens_.copy_(case["seq_lens"])
+        starts.copy_(offsets(nodes))
+        mask[:n, 1 : 1 + words].copy_(pack(matrices, words))
+        new = torch.randn(rows, hq, d, generator=torch.Generator().manual_seed(i)).bfloat16()
+        q.copy_(new)
+        out.fill_(math.nan)
+        lse.fill_(math.nan)
+        graph.replay()
+        want, want_lse, spread = reference(new[:n], case, nodes, matrices, pr, hkv, 16, d ** -0.5)
+        _check(out[:n].cpu(), lse[:n].cpu(), want, want_lse, spread)
+        assert (out[n:] == 0).all() and (lse[n:] == -math.inf).all()
+    assert ops.read_and_clear_errors(out.device) == 0
