@@ -12,11 +12,12 @@
 //     rotations fill the other's waits.  One K~ buffer is enough: keys are written during the softmax of the tile before.  V~ has
 //     two where there is room (all but two-term head_dim 128), which is worth 3 %;
 //   * warps without a draft take no part.
-// Measured (graph replays; in brackets the floor by bytes or operations), us: 8 drafts behind 1024 tokens of 28 / 4 heads of 128 21.7 (0.1);
-// 16 sequences of 300 to 8100 tokens, 5 to 24 drafts, 32 / 8 heads, fp16 108 (11.8); 64 of 4096 with 16 drafts, bf16 230 (46); 8 of
-// 65536 with 48 to 64 drafts, 32 / 32 heads of 96 1480 (268).  A call of few tiles is its chain: 13 thousand cycles of search, queries and
-// rotation, 6 of the first tile, 8 of un-rotation and stores.  In long ones a CTA takes 3000 cycles a tile: keys 1200 and values 1000 of
-// the dequantising warps, and 750 for their four waits; the softmax warps need 1600 of them, the products 530.  The load/store pipe is
+// Measured (graph replays; in brackets the floor by bytes or operations), us: 8 drafts behind 1024 tokens of 28 / 4 heads of 128 21.1 (0.1);
+// 16 sequences of 300 to 8100 tokens, 5 to 24 drafts, 32 / 8 heads, fp16 108 (11.8); 64 of 4096 with 16 drafts, bf16 223 (46); 8 of
+// 65536 with 48 to 64 drafts, 32 / 32 heads of 96 1440 (268).  A call of few tiles is its chain: 13 thousand cycles of search, queries and
+// rotation, 6 of the first tile, 8 of un-rotation and stores.  In long ones a CTA takes 2900 cycles a tile, for
+// keys and values (1200 and 1000) and the waits of the dequantising warps (750 with a wait for each of four barriers, 3050 in all and
+// 231 us at 64 x 4096); the softmax warps need 1600 of them, the products 530.  The load/store pipe is
 // 56 % busy with wavefronts and some 17 % more with operand reads and boxes: items of the same warps take twice as long with two
 // CTAs as with one.  What took work off one of the groups moved it to the other, and none of it paid: rows of fewer than 64
 // twice or four times among the 128, each with its share of a tile's columns, softmax 770 cycles a tile, 247 us instead of 234 at 64 x 4096; the
@@ -66,7 +67,11 @@ struct Cfg {
   // packed rows of a tile: K [64][D / 2], V [64][D / 2 + 16] (from the 16-byte boundary before it), the 16 bytes around each norm
   static constexpr uint32_t kVPitch = D / 2 + 16, kRawV = kBN * (D / 2), kRawKn = kRawV + kBN * kVPitch, kRawVn = kRawKn + kBN * 16;
   static constexpr uint32_t kRaw = kRawVn + kBN * 16;
+  // stages of packed rows.  With two, keys and values of a tile are asked for, waited for and given back together; with one, apart, so that
+  // the next keys are on their way while the values are being read
   static constexpr int kStages = QLO_SMEM ? 1 : 2;
+  static constexpr bool kJoint = kStages == 2;
+  static_assert(!kJoint || NVB == 2, "the keys' wait stands for the values'");
   static constexpr uint32_t kOffNorm = kOffRaw + kStages * kRaw;
   static constexpr uint32_t kSmem = kOffNorm + 2 * 2 * kBN * 4;
   // rows on their way out, padded against bank conflicts: 16-bit ones, or fp32 partials
@@ -91,7 +96,7 @@ struct Bars {
   uint64_t rawk[2], rawv[2];          // packed keys and norms / values of a stage landed
   uint64_t rawk_free[2], rawv_free[2];  // ... and read
   uint64_t kready, vready[2];         // dequantising warps -> issuer: K~ / V~ (of a buffer) written
-  uint64_t kfree, vfree[2];           // MMAs -> dequantising warps: ... read
+  uint64_t kfree, vfree;              // MMAs -> dequantising warps: ... read (vfree: where there is one buffer)
   uint64_t sready, pready;            // MMAs -> softmax: scores complete / softmax -> issuer: P written
   uint64_t img, aready, rot, qready;  // Pi's image landed / A operand of a rotation staged / rotation complete / queries in place
   uint64_t odone, drain;              // last MMA of the tile loop / of a dead CTA complete
@@ -273,10 +278,10 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
       bar_init(bar(s_bars.rawk_free[i]), kDeq / 32);
       bar_init(bar(s_bars.rawv_free[i]), kDeq / 32);
       bar_init(bar(s_bars.vready[i]), kDeq / 32);
-      bar_init(bar(s_bars.vfree[i]), 1);
     }
     bar_init(bar(s_bars.kready), kDeq / 32);
     bar_init(bar(s_bars.kfree), 1);
+    bar_init(bar(s_bars.vfree), 1);
     bar_init(bar(s_bars.sready), 1);
     bar_init(bar(s_bars.pready), row_warps);
     bar_init(bar(s_bars.img), 1);
@@ -350,14 +355,20 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
       }
       const int groups = __popc(__ballot_sync(0xffffffffu, want)) / 4;
       const unsigned bads = __ballot_sync(0xffffffffu, bad && kind == 0);
-      if (u > 0) ok = bar_wait(bar(s_bars.rawk_free[st]), (uint32_t)((u - 1) & 1), dead);
+      if (u > 0) ok = bar_wait(bar(C::kJoint ? s_bars.rawv_free[st] : s_bars.rawk_free[st]), (uint32_t)((u - 1) & 1), dead);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       if (lane == 0) {
         s_badgrp[st] = (int)((bads & 1) | (bads >> 3 & 2) | (bads >> 6 & 4) | (bads >> 9 & 8));
-        expect_tx(bar(s_bars.rawk[st]), groups * kGroup * (D / 2 + 32));
+        expect_tx(bar(s_bars.rawk[st]), groups * kGroup * (D / 2 + 32 + (C::kJoint ? C::kVPitch : 0)));
       }
       __syncwarp();
+      if (C::kJoint) {
+        if (want) box_load(dst + st * C::kRaw, map, x, in, page, bar(s_bars.rawk[st]));
+        issued = 2 * j + 1;  // (as keys)
+        page = next;
+        continue;
+      }
       if (want && kind != 1) box_load(dst + st * C::kRaw, map, x, in, page, bar(s_bars.rawk[st]));
       if (u > 0) ok = bar_wait(bar(s_bars.rawv_free[st]), (uint32_t)((u - 1) & 1), dead);
       ok = __all_sync(0xffffffffu, ok);
@@ -369,7 +380,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
     }
     // every box has landed before the CTA ends
     for (int st = 0; st < C::kStages; ++st) {
-      const int nk = (issued + 1) / 2, nv = issued / 2;  // tiles whose keys / values were asked for
+      const int nk = (issued + 1) / 2, nv = C::kJoint ? 0 : issued / 2;  // tiles whose keys / values were asked for
       const int uk = (nk - st + C::kStages - 1) / C::kStages, uv = (nv - st + C::kStages - 1) / C::kStages;  // ... into this stage
       if (uk > 0) bar_wait_own(bar(s_bars.rawk[st]), (uint32_t)((uk - 1) & 1), dead);
       if (uv > 0) bar_wait_own(bar(s_bars.rawv[st]), (uint32_t)((uv - 1) & 1), dead);
@@ -419,7 +430,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
           mma_ta(tmem + C::kColS, tmem + C::kColQ + 8 * s, db, idS, C::QLO || s > 0);
         }
         mma_commit(bar(s_bars.sready));
-        mma_commit(bar(s_bars.kfree));
+        mma_commit(bar(s_bars.kfree));  // (and of every product before)
       };
       auto issue_pv = [&](int j) {  // O += P V~
 #pragma unroll
@@ -429,7 +440,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
           if (!FAST) mma_ta(tmem + C::kColO, ph + 8, dv, idO, j > 0 || s > 0);
           mma_ta(tmem + C::kColO, ph, dv, idO, !FAST || j > 0 || s > 0);
         }
-        mma_commit(bar(s_bars.vfree[j % C::NVB]));
+        if (C::NVB == 1) mma_commit(bar(s_bars.vfree));
       };
       ok = ok && bar_wait(bar(s_bars.qready), 0u, dead);
       ok = ok && bar_wait(bar(s_bars.kready), 0u, dead);
@@ -519,21 +530,26 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
       }
     };
     const int v_off = v_at & 15, kn_off = kn_at & 15, vn_off = vn_at & 15;
-    auto done = [&](uint64_t& written, uint64_t& read) {
+    // two waits, in one round trip where both are over (in the kernel with one stage that is no gain: 16 ragged sequences 109 us, 108 without)
+    auto wait_both = [&](bool second, const uint64_t& x, uint32_t px, const uint64_t& y, uint32_t py) -> bool {
+      bool a = C::kJoint && bar_try(bar(x), px), b = !second || (C::kJoint && bar_try(bar(y), py));
+      if (!a) a = bar_wait(bar(x), px, dead);
+      if (!b) b = bar_wait(bar(y), py, dead);
+      return __all_sync(0xffffffffu, a && b);
+    };
+    auto done = [&](uint64_t& written, const uint64_t* read) {
       fence_async();
       __syncwarp();
       if (lane == 0) {
         bar_arrive(bar(written));
-        bar_arrive(bar(read));
+        if (read) bar_arrive(bar(*read));
       }
     };
     for (int j = 0; j < n_tiles && ok; ++j) {
       const int st = j % C::kStages, u = j / C::kStages;
       const unsigned char* raw = sm + C::kOffRaw + st * C::kRaw;
       // ---- keys and norms ------------------------------------------------------------------------------------
-      ok = bar_wait(bar(s_bars.rawk[st]), (uint32_t)(u & 1), dead);
-      if (j > 0) ok = ok && bar_wait(bar(s_bars.kfree), (uint32_t)((j - 1) & 1), dead);
-      ok = __all_sync(0xffffffffu, ok);
+      ok = wait_both(j > 0, s_bars.rawk[st], (uint32_t)(u & 1), s_bars.kfree, (uint32_t)((j - 1) & 1));
       if (!ok) break;
       if (t < kBN) {
         float* ns = reinterpret_cast<float*>(sm + C::kOffNorm) + (j & 1) * 2 * kBN;
@@ -550,11 +566,11 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
         int tok, seg;
         if (item(n, tok, seg)) expand(*reinterpret_cast<const uint4*>(raw + tok * (D / 2) + 16 * seg), lut_k, C::kOffK, tok, seg);
       }
-      done(s_bars.kready, s_bars.rawk_free[st]);
+      done(s_bars.kready, C::kJoint ? nullptr : &s_bars.rawk_free[st]);
       // ---- values ----------------------------------------------------------------------------------------------
-      ok = bar_wait(bar(s_bars.rawv[st]), (uint32_t)(u & 1), dead);
-      if (j >= C::NVB) ok = ok && bar_wait(bar(s_bars.vfree[j % C::NVB]), (uint32_t)((j / C::NVB - 1) & 1), dead);
-      ok = __all_sync(0xffffffffu, ok);
+      // (With two buffers: that the keys' buffer is free says that S of the tile before is complete, and with it the products with V~ that
+      // were asked for in front of it, those of two tiles ago.)
+      if (!C::kJoint) ok = wait_both(j >= C::NVB, s_bars.rawv[st], (uint32_t)(u & 1), s_bars.vfree, (uint32_t)((j / C::NVB - 1) & 1));
       if (!ok) break;
 #pragma unroll
       for (int n = 0; n < NIT; ++n) {
@@ -571,7 +587,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
           expand(x, lut_v, C::kOffV + (j % C::NVB) * C::kKv, tok, seg);
         }
       }
-      done(s_bars.vready[j % C::NVB], s_bars.rawv_free[st]);
+      done(s_bars.vready[j % C::NVB], &s_bars.rawv_free[st]);
     }
   } else {
     // ================= softmax warps: a row per thread =================
