@@ -481,3 +481,21 @@ def test_a_replayed_graph_follows_lengths_offsets_and_masks(ops, d, hq, hkv):
         _check(out[:n].cpu(), lse[:n].cpu(), want, want_lse, spread)
         assert (out[n:] == 0).all() and (lse[n:] == -math.inf).all()
     assert ops.read_and_clear_errors(out.device) == 0
+
+
+@pytest.mark.parametrize("lens,nodes", [([100], [20]), ([3000, 70], [30, 3]), ([400], [200])])  # one part, parts of the keys, many drafts
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("bad", [math.inf, math.nan])
+def test_a_query_that_is_not_finite_is_its_own_rows_alone(ops, lens, nodes, dtype, bad):
+    pr = Prims(128)
+    case = build_paged_case(lens, 2, 128, 16, pr, seed=6, padded=True)
+    mask = pack(ancestor_matrix(nodes, random_parents(nodes, random.Random(2), 3)), -(-max(nodes) // 32))
+    q = torch.randn(sum(nodes), 8, 128, generator=torch.Generator().manual_seed(3)).to(DTYPES[dtype])
+    good = _call(ops, q, case, nodes, mask, pr.cuda(), 2, 16)
+    hit = torch.zeros(sum(nodes), 8, dtype=torch.bool)
+    hit[4, 5] = hit[17, 0] = True
+    q[hit] = q[hit].clone().index_fill_(1, torch.tensor([9]), bad)
+    got = _call(ops, q, case, nodes, mask, pr.cuda(), 2, 16)
+    assert torch.isnan(got.cpu()[hit]).all()  # (an infinite coordinate makes scores of both signs, and the rotation of it NaN)
+    assert torch.equal(got.cpu()[~hit], good.cpu()[~hit])
+    assert ops.read_and_clear_errors(got.device) == 0
