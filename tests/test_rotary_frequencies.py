@@ -107,3 +107,28 @@ def test_status_of_the_c_entry_points_without_a_launch(cuda_lib):
     assert lib.tq4_compact_rows(at, 1, 8, 16, 16 * 272, 272, 2, 128, at, 4, 4, 2, at, at, 65, 65, at, None, None, 0, None, None) == workspace
     assert lib.tq4_compact_rows(at, 1, 8, 16, 16 * 272, 272, 2, 128, at, 4, 4, 2, None, at, 5, 5, at, None, None, 0, None, None) == invalid
     assert lib.tq4_tree_attention_workspace_bytes(0, 8, 2, 128) == 0 and lib.tq4_tree_attention_workspace_bytes(5, 8, 2, 100) == 0
+
+
+@pytest.mark.parametrize("longest,extra", [(131072, {}), (131072, {"factor": 8.0}), (131072, {"attention_factor": 1.3}), (4096, {}), (2048, {})])
+@pytest.mark.parametrize("seq_len", [None, 100, 20000])
+def test_longrope_takes_its_factor_from_the_longest_context(longest, extra, seq_len):
+    """A configuration as Phi-3 models carry it: lists of factors and the original context, no ``factor``."""
+    from transformers import Phi3Config
+    from transformers.modeling_rope_utils import ROPE_INIT_FUNCTIONS
+
+    scaling = {"rope_type": "longrope", "rope_theta": 10000.0, "short_factor": [1.0 + i / 64 for i in range(48)],
+               "long_factor": [2.0 + i for i in range(48)], **extra}
+    config = Phi3Config(hidden_size=96 * 4, num_attention_heads=4, num_key_value_heads=4, max_position_embeddings=longest,
+                        original_max_position_embeddings=4096, rope_parameters=scaling, pad_token_id=0)
+    assert config.rope_parameters["original_max_position_embeddings"] == 4096 and ("factor" in config.rope_parameters) == ("factor" in extra)
+    want, want_factor = ROPE_INIT_FUNCTIONS["longrope"](config, torch.device("cpu"), seq_len=seq_len)
+    got, factor = rotary_inv_freq(96, 10000.0, config.rope_parameters, seq_len=seq_len, max_position_embeddings=longest)
+    assert torch.allclose(got.float(), want.float(), rtol=16 * 2 ** -24, atol=0)
+    assert math.isclose(factor, want_factor, rel_tol=1e-12)
+
+
+def test_longrope_without_anything_that_gives_its_factor_is_refused():
+    scaling = {"rope_type": "longrope", "short_factor": [1.0] * 48, "long_factor": [2.0] * 48, "original_max_position_embeddings": 4096}
+    with pytest.raises(ValueError, match="max_position_embeddings"):
+        rotary_inv_freq(96, scaling=scaling)
+    assert rotary_inv_freq(96, scaling={**scaling, "attention_factor": 1.0})[1] == 1.0

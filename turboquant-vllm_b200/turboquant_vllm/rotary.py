@@ -53,16 +53,18 @@ def rotary_inv_freq(
     scaling: dict[str, Any] | None = None,
     *,
     seq_len: int | None = None,
+    max_position_embeddings: int | None = None,
     device: torch.device | str | None = None,
 ) -> tuple[torch.Tensor, float]:
     """``(inv_freq fp64 [rotary_dim / 2], attention_factor)`` for ``tq4_rotary``.
 
     ``scaling["rope_type"]`` (or ``"type"``): ``default``, ``linear`` (positions divided by ``factor``), ``dynamic`` (the base grows with
     ``seq_len`` beyond ``original_max_position_embeddings``), ``yarn``, ``llama3`` or ``longrope`` (``short_factor`` / ``long_factor`` per
-    frequency, by ``seq_len``).
+    frequency, by ``seq_len``).  ``max_position_embeddings``: the configuration's longest context, from which ``longrope`` takes the factor
+    that its attention factor follows from, where the dictionary holds neither (as those of Phi-3 models do not).
 
     Raises:
-        ValueError: ``rotary_dim`` is not even and positive, or the type is unknown.
+        ValueError: ``rotary_dim`` is not even and positive, the type is unknown, or nothing gives the attention factor of ``longrope``.
     """
     if rotary_dim <= 0 or rotary_dim % 2:
         raise ValueError(f"rotary_dim must be even and positive, got {rotary_dim}")
@@ -93,7 +95,10 @@ def rotary_inv_freq(
         inv_freq = inv_freq / per
         attention = scaling.get("attention_factor")
         if attention is None:
-            factor = float(scaling.get("factor") or 1.0)
+            factor = scaling.get("factor")
+            if factor is None and max_position_embeddings is None:
+                raise ValueError("longrope scaling needs factor, attention_factor or max_position_embeddings")
+            factor = float(factor) if factor is not None else max_position_embeddings / original
             attention = 1.0 if factor <= 1 else math.sqrt(1 + math.log(factor) / math.log(original))
     elif kind not in ("default", "dynamic"):
         raise ValueError(f"unknown rotary scaling {kind!r}")
