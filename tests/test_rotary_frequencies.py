@@ -132,3 +132,22 @@ def test_longrope_without_anything_that_gives_its_factor_is_refused():
     with pytest.raises(ValueError, match="max_position_embeddings"):
         rotary_inv_freq(96, scaling=scaling)
     assert rotary_inv_freq(96, scaling={**scaling, "attention_factor": 1.0})[1] == 1.0
+
+
+NEEDED = {
+    "linear": ["factor"],
+    "dynamic": ["factor", "original_max_position_embeddings"],
+    "yarn": ["factor", "original_max_position_embeddings"],
+    "llama3": ["factor", "low_freq_factor", "high_freq_factor", "original_max_position_embeddings"],
+    "longrope": ["original_max_position_embeddings", "short_factor", "long_factor"],
+}
+
+
+@pytest.mark.parametrize("kind,key", [(kind, key) for kind, keys in NEEDED.items() for key in keys])
+@pytest.mark.parametrize("absent", [False, True])
+def test_a_dictionary_without_a_key_that_its_type_needs_is_refused_by_name(kind, key, absent):
+    scaling = {"rope_type": kind, "low_freq_factor": 1.0, "high_freq_factor": 4.0, **SCALINGS[kind], key: None}
+    if absent:
+        del scaling[key]
+    with pytest.raises(ValueError, match=f"{kind}.*{key}"):
+        rotary_inv_freq(128, scaling=scaling, seq_len=None if key == "short_factor" else 20000)

@@ -12,11 +12,18 @@ from typing import Any
 import torch
 
 
+def _needed(scaling: dict[str, Any], kind: str, key: str) -> Any:
+    value = scaling.get(key)
+    if value is None:
+        raise ValueError(f"{kind} scaling needs {key}")
+    return value
+
+
 def _yarn(inv_freq: torch.Tensor, dim: int, base: float, scaling: dict[str, Any]) -> tuple[torch.Tensor, float]:
     """Frequencies that turn often over the original context stay, those that turn rarely are divided by the factor, with a ramp
     between the two (Peng et al., "YaRN", section 3); the attention factor is that of their equation 22."""
-    factor = float(scaling["factor"])
-    original = float(scaling["original_max_position_embeddings"])
+    factor = float(_needed(scaling, "yarn", "factor"))
+    original = float(_needed(scaling, "yarn", "original_max_position_embeddings"))
 
     def place(turns: float) -> float:  # of the frequency that makes so many turns over the original context
         return dim * math.log(original / (turns * 2 * math.pi)) / (2 * math.log(base))
@@ -40,8 +47,8 @@ def _yarn(inv_freq: torch.Tensor, dim: int, base: float, scaling: dict[str, Any]
 def _llama3(inv_freq: torch.Tensor, scaling: dict[str, Any]) -> torch.Tensor:
     """Wavelengths up to a share of the original context stay, those beyond another are stretched by the factor, linear in the
     number of turns between."""
-    factor, original = float(scaling["factor"]), float(scaling["original_max_position_embeddings"])
-    low, high = float(scaling["low_freq_factor"]), float(scaling["high_freq_factor"])
+    factor, original, low, high = (float(_needed(scaling, "llama3", key)) for key in (
+        "factor", "original_max_position_embeddings", "low_freq_factor", "high_freq_factor"))
     turns = original * inv_freq / (2 * math.pi)
     keep = ((turns - low) / (high - low)).clamp(0, 1)
     return inv_freq * (keep + (1 - keep) / factor)
@@ -64,7 +71,8 @@ def rotary_inv_freq(
     that its attention factor follows from, where the dictionary holds neither (as those of Phi-3 models do not).
 
     Raises:
-        ValueError: ``rotary_dim`` is not even and positive, the type is unknown, or nothing gives the attention factor of ``longrope``.
+        ValueError: ``rotary_dim`` is not even and positive, the type is unknown, or a key that the type needs is missing (for ``longrope``: all
+            that could give its attention factor).
     """
     if rotary_dim <= 0 or rotary_dim % 2:
         raise ValueError(f"rotary_dim must be even and positive, got {rotary_dim}")
@@ -74,22 +82,20 @@ def rotary_inv_freq(
     exponent = torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim
     attention = 1.0
     if kind == "dynamic":
-        original = scaling.get("original_max_position_embeddings")
-        if original is None:
-            raise ValueError("dynamic scaling needs original_max_position_embeddings")
-        factor, length = float(scaling["factor"]), max(seq_len or 0, original)
+        original = _needed(scaling, kind, "original_max_position_embeddings")
+        factor, length = float(_needed(scaling, kind, "factor")), max(seq_len or 0, original)
         base *= (factor * length / original - (factor - 1)) ** (rotary_dim / (rotary_dim - 2))
     inv_freq = base ** -exponent
     if kind == "linear":
-        inv_freq = inv_freq / float(scaling["factor"])
+        inv_freq = inv_freq / float(_needed(scaling, kind, "factor"))
     elif kind == "yarn":
         inv_freq, attention = _yarn(inv_freq, rotary_dim, base, scaling)
     elif kind == "llama3":
         inv_freq = _llama3(inv_freq, scaling)
     elif kind == "longrope":
-        original = scaling["original_max_position_embeddings"]
+        original = _needed(scaling, kind, "original_max_position_embeddings")
         far = seq_len is not None and seq_len > original
-        per = torch.tensor(scaling["long_factor" if far else "short_factor"], dtype=torch.float64)
+        per = torch.tensor(_needed(scaling, kind, "long_factor" if far else "short_factor"), dtype=torch.float64)
         if per.shape != inv_freq.shape:
             raise ValueError(f"longrope needs {inv_freq.numel()} factors, got {per.numel()}")
         inv_freq = inv_freq / per
