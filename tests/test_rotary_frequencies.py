@@ -151,3 +151,10 @@ def test_a_dictionary_without_a_key_that_its_type_needs_is_refused_by_name(kind,
         del scaling[key]
     with pytest.raises(ValueError, match=f"{kind}.*{key}"):
         rotary_inv_freq(128, scaling=scaling, seq_len=None if key == "short_factor" else 20000)
+
+
+def test_dynamic_scaling_of_a_single_pair_is_refused():
+    """The exponent of its base is rotary_dim / (rotary_dim - 2)."""
+    with pytest.raises(ValueError, match="dynamic.*rotary_dim"):
+        rotary_inv_freq(2, scaling={"rope_type": "dynamic", "factor": 2.0, "original_max_position_embeddings": 2048})
+    assert rotary_inv_freq(4, scaling={"rope_type": "dynamic", "factor": 2.0, "original_max_position_embeddings": 2048})[0].shape == (2,)

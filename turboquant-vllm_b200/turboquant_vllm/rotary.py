@@ -82,6 +82,8 @@ def rotary_inv_freq(
     exponent = torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim
     attention = 1.0
     if kind == "dynamic":
+        if rotary_dim == 2:
+            raise ValueError("dynamic scaling needs a rotary_dim of 4 or more")
         original = _needed(scaling, kind, "original_max_position_embeddings")
         factor, length = float(_needed(scaling, kind, "factor")), max(seq_len or 0, original)
         base *= (factor * length / original - (factor - 1)) ** (rotary_dim / (rotary_dim - 2))
