@@ -499,3 +499,50 @@ def test_a_query_that_is_not_finite_is_its_own_rows_alone(ops, lens, nodes, dtyp
     assert torch.isnan(got.cpu()[hit]).all()  # (an infinite coordinate makes scores of both signs, and the rotation of it NaN)
     assert torch.equal(got.cpu()[~hit], good.cpu()[~hit])
     assert ops.read_and_clear_errors(got.device) == 0
+
+
+@pytest.mark.parametrize("d,hq,hkv,lens,nodes", [
+    (128, 8, 2, [100], [20]), (128, 8, 2, [3000, 70], [30, 3]), (128, 8, 2, [400], [200]),  # one part, parts of the keys, many drafts
+    (256, 8, 4, [100], [20]), (256, 8, 4, [3000], [12]), (96, 4, 4, [2000], [9])])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("where", ["key", "value", "query"])
+@pytest.mark.parametrize("bad", [math.inf, math.nan])
+def test_the_lse_of_a_row_that_is_not_finite_is_nan(ops, d, hq, hkv, lens, nodes, dtype, where, bad):
+    """Whether or not the keys are cut; and a merge with another part of the context hands it on instead of leaving the row's keys out."""
+    pr, bs = Prims(d), 16
+    p = pr.cuda()
+    case = build_paged_case(lens, hkv, d, bs, pr, seed=6, padded=True)
+    other = build_paged_case([200, 50][: len(lens)], hkv, d, bs, pr, seed=7, padded=True)
+    matrices = ancestor_matrix(nodes, random_parents(nodes, random.Random(2), 3))
+    mask = pack(matrices, -(-max(nodes) // 32))
+    q = torch.randn(sum(nodes), hq, d, generator=torch.Generator().manual_seed(3)).to(DTYPES[dtype])
+
+    def run(q, case):
+        lse = torch.zeros(sum(nodes), hq, device="cuda")
+        out = _call(ops, q, case, nodes, mask, p, hkv, bs, out_dtype=torch.float32, out_rotated=True, lse_out=lse)
+        return out, lse
+
+    good, good_lse = run(q, case)
+    healthy, healthy_lse = run(q, other)
+    assert torch.isfinite(good_lse).all() and torch.isfinite(healthy_lse).all()
+    hit = torch.zeros(sum(nodes), hq, dtype=torch.bool)
+    if where == "query":
+        hit[4, hq - 1] = hit[8, 0] = True
+        hurt_q, hurt = q.clone(), case
+        hurt_q[hit] = q[hit].index_fill(1, torch.tensor([9]), bad)
+    else:
+        hurt_q, hurt = q, dict(case, cache=case["cache"].clone())
+        token = lens[0] - nodes[0] + 4
+        at = hkv * d // 2 if where == "key" else hkv * d + 4 * hkv
+        row = hurt["cache"][case["block_table"][0, token // bs].long(), token % bs]
+        row[at : at + 4] = torch.tensor([bad]).view(torch.uint8)  # (the first KV head's)
+        hit[: nodes[0], : hq // hkv] = torch.from_numpy(matrices[0][:, 4])[:, None]
+        assert hit.any() and not hit.all()
+    hit = hit.cuda()
+    got, lse = run(hurt_q, hurt)
+    assert torch.isnan(got[hit]).all() and torch.equal(got[~hit], good[~hit])
+    assert torch.isnan(lse[hit]).all() and torch.equal(lse[~hit], good_lse[~hit])
+    merged = ops.combine_partials(torch.stack((got, healthy)), torch.stack((lse, healthy_lse)), p["rot"])
+    want = ops.combine_partials(torch.stack((good, healthy)), torch.stack((good_lse, healthy_lse)), p["rot"])
+    assert torch.isnan(merged[hit]).all() and torch.equal(merged[~hit], want[~hit])
+    assert ops.read_and_clear_errors(got.device) == 0

@@ -1028,7 +1028,7 @@ __global__ void __launch_bounds__(256) combine_kernel(const CombineArgs a) {
           wu[u] = exp2f(s_m[v * WPV + u] - m_use);
           L = fmaf(s_l[v * WPV + u], wu[u], L);
         }
-        const float inv = L > 0.f ? 1.f / L : 0.f;
+        const float inv = L != 0.f ? 1.f / L : 0.f;  // (NaN: handed on)
         // the warps of a vector share its coordinates
         for (int d = sub * 32 + lane; d < D; d += 32 * WPV) {
           float x = 0.f;
@@ -1037,7 +1037,7 @@ __global__ void __launch_bounds__(256) combine_kernel(const CombineArgs a) {
           s_x[v * C::XP + d] = x * inv;
         }
       } else {
-        const float inv = L > 0.f ? 1.f / L : 0.f;
+        const float inv = L != 0.f ? 1.f / L : 0.f;  // (NaN: handed on)
 #pragma unroll
         for (int r = 0; r < R; ++r)
           if (4 * lane + 128 * r < D)
@@ -1046,7 +1046,7 @@ __global__ void __launch_bounds__(256) combine_kernel(const CombineArgs a) {
       }
       if (a.lse_out && split == 0 && sub == 0 && lane == 0 && vec < n_vec && row_mine(vec / a.Hq))
         a.lse_out[(int64_t)a.row_offset * a.Hq + vec] =
-            L > 0.f ? (M + log2f(L)) * 0.6931471805599453f : -CUDART_INF_F;
+            L != 0.f ? (M + log2f(L)) * 0.6931471805599453f : -CUDART_INF_F;
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();
