@@ -118,3 +118,31 @@ def test_which_calls_take_it(cuda_lib, d, rows, keys, steps):
     a, ma = _run(ops, nv, (q, case["cache"].cuda(), table[:, : keys // 16].contiguous().cuda(), *rest))
     b, mb = _run(ops, nv, (q, case["cache"].cuda(), table.cuda(), *rest), max_seq_len=keys)
     assert ma == mb == 1 - steps and torch.equal(a, b)
+
+
+@pytest.mark.parametrize("d,hq,hkv,lens", [(128, 8, 2, [100, 700]), (256, 8, 4, [300]), (64, 14, 2, [60, 90])])
+@pytest.mark.parametrize("where", ["key", "value", "query"])
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+def test_a_row_that_is_not_finite_is_not_one_without_keys(cuda_lib, d, hq, hkv, lens, where, bad):
+    """An lse of -inf is what a row without keys has: a merge would leave out the row's keys.  As in the streaming kernel."""
+    from turboquant_vllm import _native as nv
+    from turboquant_vllm.kernels import ops
+
+    pr = Prims(d)
+    p = pr.cuda()
+    case = build_paged_case(lens, hkv, d, 16, pr, seed=5, padded=True)
+    q = torch.randn(len(lens), hq, d, generator=torch.Generator().manual_seed(1)).half()
+    if where == "query":
+        q[0, 0, 9] = bad
+    else:
+        at = hkv * d // 2 if where == "key" else hkv * d + 4 * hkv
+        row = case["cache"][case["block_table"][0, 3].long(), 5]
+        row[at : at + 4] = torch.tensor([bad]).view(torch.uint8)
+    args = (q.cuda(), case["cache"].cuda(), case["block_table"].cuda(), case["seq_lens"].cuda(), p["kc"], p["vc"], p["rot"], hkv, 16)
+    for mode in (0, 2):
+        lse = torch.empty(len(lens), hq, device="cuda")
+        out, merges = _run(ops, nv, args, mode=mode, lse_out=lse, out_rotated=True, out_dtype=torch.float32)
+        assert merges == (mode == 2)
+        hit = torch.isnan(out).any(dim=-1)
+        assert hit[0].any() and not hit[1:].any()
+        assert (lse > float("-inf"))[~hit].all() and not torch.isinf(lse[hit]).any()

@@ -478,10 +478,10 @@ decode_step_kernel(const __grid_constant__ AttnArgs a, const int cl_shift) {
       o.x = fmaf(x.x, e, o.x); o.y = fmaf(x.y, e, o.y); o.z = fmaf(x.z, e, o.z); o.w = fmaf(x.w, e, o.w);
     }
     if (cl == 1) {
-      const float inv = L > 0.f ? 1.f / L : 0.f;
+      const float inv = L != 0.f ? 1.f / L : 0.f;
       *reinterpret_cast<float4*>(s_x + h * D + d) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
       if (d == 0 && a.lse_out)
-        a.lse_out[((int64_t)r + sh.row_offset) * sh.Hq + qh0 + h] = L > 0.f ? (M + log2f(L)) * 0.6931471805599453f : -CUDART_INF_F;
+        a.lse_out[((int64_t)r + sh.row_offset) * sh.Hq + qh0 + h] = L != 0.f ? (M + log2f(L)) * 0.6931471805599453f : -CUDART_INF_F;  // (NaN: handed on)
     } else {
       const uint32_t at = smem_u32(s_all + (rank * GC + h) * D + d), at_ml = smem_u32(&s_ml[rank][h]);
 #pragma unroll 4
@@ -510,10 +510,10 @@ decode_step_kernel(const __grid_constant__ AttnArgs a, const int cl_shift) {
         L = fmaf(ml.y, e, L);
         o.x = fmaf(x.x, e, o.x); o.y = fmaf(x.y, e, o.y); o.z = fmaf(x.z, e, o.z); o.w = fmaf(x.w, e, o.w);
       }
-      const float inv = L > 0.f ? 1.f / L : 0.f;
+      const float inv = L != 0.f ? 1.f / L : 0.f;
       *reinterpret_cast<float4*>(s_x + h * D + d) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
       if (d == 0 && rank == 0 && a.lse_out)
-        a.lse_out[((int64_t)r + sh.row_offset) * sh.Hq + qh0 + h] = L > 0.f ? (M + log2f(L)) * 0.6931471805599453f : -CUDART_INF_F;
+        a.lse_out[((int64_t)r + sh.row_offset) * sh.Hq + qh0 + h] = L != 0.f ? (M + log2f(L)) * 0.6931471805599453f : -CUDART_INF_F;  // (NaN: handed on)
     }
   }
   __syncthreads();
