@@ -49,7 +49,8 @@ typedef enum {
 #define TQ4_DEV_BAD_SLOT 1  /* slot_mapping entry >= num_cache_slots            */
 #define TQ4_DEV_BAD_BLOCK 2 /* block_table entry outside [0, num_blocks), or a seq_len beyond the
                                bt_stride * block_size tokens a block-table row can address (cut there) */
-#define TQ4_DEV_TIMEOUT 4   /* a bounded device-side wait gave up                */
+#define TQ4_DEV_TIMEOUT 4   /* a bounded device-side wait gave up: the call's results are not to be used
+                               (tq4_compact_rows has then moved some rows and may have overwritten others) */
 #define TQ4_DEV_WRITE_ORDER 8 /* tq4_write_and_attention: a new token's slot is not the last position of its
                                  sequence; it was written, but this call's attention may not have seen it */
 #define TQ4_DEV_PAGE_CONFLICT 16 /* tq4_copy_blocks: a page is the destination of two pairs with different sources, or

@@ -75,6 +75,19 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity) {
   }
   return false;
 }
+__device__ __forceinline__ void bar_fence() { asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory"); }
+// The mark of a segment of rows says that they have been loaded; a bounded wait for one.
+__device__ __forceinline__ void mark_set(int* mark) { asm volatile("st.release.gpu.global.s32 [%0], 1;" ::"l"(mark) : "memory"); }
+__device__ __forceinline__ bool mark_wait(const int* mark) {
+  for (int it = 0; it < (1 << 20); ++it) {
+    int there;
+    asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(there) : "l"(mark) : "memory");
+    if (there) return true;
+  }
+  return false;
+}
+// marks are read like any memory, what bulk copies write is not
+__device__ __forceinline__ void mark_fence() { asm volatile("fence.proxy.async.global;" ::: "memory"); }
 
 // ======================================================================================
 // Pages copied
@@ -173,7 +186,7 @@ __global__ void __launch_bounds__(32) copy_blocks_bulk_kernel(const __grid_const
   const int64_t src = index_at(a.pairs, a.pairs_64, 2 * pair), dst = index_at(a.pairs, a.pairs_64, 2 * pair + 1);
   const uint32_t bytes = (uint32_t)a.g.row_units * 16, slot = smem_of(s_rows) + lane * bytes;
   if (lane < kStages) bar_init(smem_of(&s_bar[lane]));
-  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  bar_fence();
   __syncwarp();
   if (!pair_counts(a, pair, src, dst)) return;
   const int sets = (a.g.block_size + a.rows - 1) / a.rows, all = sets * layers;  // of a page; of the block
@@ -189,18 +202,20 @@ __global__ void __launch_bounds__(32) copy_blocks_bulk_kernel(const __grid_const
     __syncwarp();
     if (lane < n) bulk_in(slot + (i % kStages) * stage, at(i, src), bytes, bar);
   };
-  for (int i = 0; i < min(kStages, all); ++i) ask(i);
+  auto landed = [&](int i) { return bar_wait(smem_of(&s_bar[i % kStages]), (i / kStages) & 1); };
+  int asked = 0;
+  while (asked < min(kStages, all)) ask(asked++);
   for (int i = 0; i < all; ++i) {
-    if (!bar_wait(smem_of(&s_bar[i % kStages]), (i / kStages) & 1)) {
-      report(a.err_flag, TQ4_DEV_TIMEOUT);
-      for (int k = i + 1; k < min(i + kStages, all); ++k) bar_wait(smem_of(&s_bar[k % kStages]), (k / kStages) & 1);  // (copies under way)
+    if (!__all_sync(0xffffffffu, landed(i))) {
+      if (lane == 0) report(a.err_flag, TQ4_DEV_TIMEOUT);
+      for (int k = i; k < asked; ++k) landed(k);  // (copies under way: the shared memory is another CTA's after this one)
       break;
     }
     if (lane < rows_of(i)) bulk_out(at(i, dst), slot + (i % kStages) * stage, bytes);
     bulk_commit();
-    if (i > 0 && i - 1 + kStages < all) {
+    if (i > 0 && asked < all) {
       bulk_wait_read<1>();
-      ask(i - 1 + kStages);
+      ask(asked++);
     }
   }
   bulk_wait_all();
@@ -321,7 +336,7 @@ __global__ void __launch_bounds__(32) compact_short_bulk_kernel(const __grid_con
     bar_init(bar);
     if (layer0 == 0 && a.lens_out) a.lens_out[seq] = a.first[seq] + a.kept[seq];
   }
-  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  bar_fence();
   int bad = n < 0;
   for (int j = lane; j < n; j += 32) bad |= keep[j] < 0 || (j > 0 && keep[j - 1] >= keep[j]);
   if (__any_sync(0xffffffffu, bad)) {  // a list out of order: reported, the sequence is left as it is
@@ -344,11 +359,11 @@ __global__ void __launch_bounds__(32) compact_short_bulk_kernel(const __grid_con
       bulk_wait_read<0>();  // (the lane's row before is out of its place)
       bulk_in(slot, caches.at[layer0 + layer] + src, bytes, bar);
     }
-    if (!bar_wait(bar, phase)) {
-      report(a.err_flag, TQ4_DEV_TIMEOUT);
+    if (!__all_sync(0xffffffffu, bar_wait(bar, phase))) {
+      if (lane == 0) report(a.err_flag, TQ4_DEV_TIMEOUT);
+      bar_wait(bar, phase);  // (copies under way: the shared memory is another CTA's after this one)
       break;
     }
-    __syncwarp();
     if (moves) bulk_out(caches.at[layer0 + layer] + dst, slot, bytes);
     bulk_commit();
   }
@@ -446,15 +461,11 @@ __global__ void __launch_bounds__(kThreads) compact_long_kernel(const __grid_con
   int* loaded = a.loaded + ((int64_t)layer * a.seqs + seq) * a.segments;
   if (tid == 0) {
     __threadfence();
-    asm volatile("st.release.gpu.global.s32 [%0], 1;" ::"l"(loaded + seg) : "memory");
+    mark_set(loaded + seg);
   }
   if (s_range[0] < s_range[1]) {
-    for (int s = s_range[0] / a.seg_rows + tid; s <= (s_range[1] - 1) / a.seg_rows; s += kThreads) {
-      int there = 0;
-      for (int it = 0; it < (1 << 20) && !there; ++it)
-        asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(there) : "l"(loaded + s) : "memory");
-      if (!there) s_stuck = 1;
-    }
+    for (int s = s_range[0] / a.seg_rows + tid; s <= (s_range[1] - 1) / a.seg_rows; s += kThreads)
+      if (!mark_wait(loaded + s)) s_stuck = 1;
     __threadfence();
     __syncthreads();
     if (s_stuck) {
@@ -477,7 +488,7 @@ __global__ void __launch_bounds__(32) compact_long_bulk_kernel(const __grid_cons
   const int lane = threadIdx.x;
   const uint32_t bar = smem_of(&s_bar), bytes = (uint32_t)a.g.row_units * 16, slot = smem_of(s_rows) + lane * bytes;
   if (lane == 0) bar_init(bar);
-  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  bar_fence();
   __syncwarp();
   pdl_wait();
   int ticket = 0;
@@ -506,22 +517,21 @@ __global__ void __launch_bounds__(32) compact_long_bulk_kernel(const __grid_cons
   if (moves) bulk_in(slot, cache + src, bytes, bar);
   // rows k < j0 that come from the places of this block's rows, and the segments that have them
   const int k0 = lower_bound_warp(keep, j0, j0, lane), k1 = lower_bound_warp(keep, j0, j0 + rows, lane);
-  bool ok = bar_wait(bar, 0);
+  if (!__all_sync(0xffffffffu, bar_wait(bar, 0))) {  // no mark: nobody overwrites what has not been read
+    if (lane == 0) report(a.err_flag, TQ4_DEV_TIMEOUT);
+    bar_wait(bar, 0);  // (copies under way: the shared memory is another CTA's after this one)
+    return;
+  }
   int* loaded = a.loaded + ((int64_t)layer * a.seqs + seq) * a.segments;
-  __syncwarp();
-  if (lane == 0) asm volatile("st.release.gpu.global.s32 [%0], 1;" ::"l"(loaded + seg) : "memory");
+  bool ok = true;
+  if (lane == 0) mark_set(loaded + seg);
   if (k0 < k1)
-    for (int s = k0 / a.seg_rows + lane; s <= (k1 - 1) / a.seg_rows; s += 32) {
-      int there = 0;
-      for (int it = 0; it < (1 << 20) && !there; ++it)
-        asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(there) : "l"(loaded + s) : "memory");
-      ok = ok && there;
-    }
+    for (int s = k0 / a.seg_rows + lane; s <= (k1 - 1) / a.seg_rows; s += 32) ok = mark_wait(loaded + s) && ok;
   if (!__all_sync(0xffffffffu, ok)) {
     if (lane == 0) report(a.err_flag, TQ4_DEV_TIMEOUT);
     return;
   }
-  asm volatile("fence.proxy.async.global;" ::: "memory");  // the marks were read like any memory, the copies are not
+  mark_fence();
   if (moves) bulk_out(cache + dst, slot, bytes);
   bulk_commit();
   bulk_wait_all();
