@@ -392,10 +392,12 @@ int tq4_tree_mask(const int32_t* parents, const int32_t* query_start_loc, int64_
  * of its set bits, minus 1, and of the former it sees those within the window; the drafts are the mask's alone.
  * tree_mask int32 [num_rows, tree_mask_words] and block_table int32 [num_seqs, bt_width] with row strides in elements; a sequence
  * longer than its row of the table is cut there (TQ4_DEV_BAD_BLOCK).  max_seq_len as in tq4_attention_step; the other arguments,
- * checks and the precision are those of tq4_paged_attention in the prefill form, with at most 128 query heads per KV head; but a call
- * with bf16 queries, a bf16 output and no lse_out may round rotated queries and weights to fp16 (4e-4 of relative 2-norm, beside the
- * output's own 1.7e-3).  A row that sees no key, or past the last offset, gets zeros and an lse of -inf.  An
- * infinite or NaN norm in the cache makes the rows that see its token NaN, and no others.
+ * checks and the precision are those of tq4_paged_attention in the prefill form, with at most 128 query heads per KV head.  mode: 0 or 3,
+ * queries and probabilities enter the tensor cores as two fp16 terms; 4 (bf16 queries; never chosen by 0), as single ones, and Pi with
+ * them: less tensor work, and an error that grows with the scores, 5e-4 of relative 2-norm where they have a standard deviation
+ * of 2, 9e-4 at 7, 2e-3 at 28 (a bf16 output's own rounding: 1.7e-3).
+ * A row that sees no key, or past the last offset, gets zeros and an lse of -inf.  An infinite or NaN norm in the cache makes the rows
+ * that see its token NaN, output and lse, and no others.
  * workspace >= tq4_tree_attention_workspace_bytes(num_rows, Hq, Hkv, D), 16-byte aligned.
  */
 size_t tq4_tree_attention_workspace_bytes(int64_t max_query_rows, int num_q_heads, int num_kv_heads, int head_dim);
@@ -412,7 +414,7 @@ int tq4_tree_attention(const void* q, int q_dtype, int64_t num_rows, int num_seq
                        const float* rotation, float sm_scale, int sliding_window,
                        void* out, int out_dtype, int64_t out_token_stride, int64_t out_head_stride,
                        float* lse_out, int out_rotated,
-                       void* workspace, size_t workspace_bytes, int* err_flag, void* stream);
+                       void* workspace, size_t workspace_bytes, int mode, int* err_flag, void* stream);
 
 /*
  * Pages copied inside the caches of all layers (no counterpart in the reference): for every pair (source, destination) the token rows

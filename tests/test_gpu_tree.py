@@ -546,3 +546,65 @@ def test_the_lse_of_a_row_that_is_not_finite_is_nan(ops, d, hq, hkv, lens, nodes
     want = ops.combine_partials(torch.stack((good, healthy)), torch.stack((good_lse, healthy_lse)), p["rot"])
     assert torch.isnan(merged[hit]).all() and torch.equal(merged[~hit], want[~hit])
     assert ops.read_and_clear_errors(got.device) == 0
+
+
+FORMS = [  # head_dim, q heads, KV heads, lengths, drafts
+    (128, 8, 2, [100, 70], [20, 3]), (128, 8, 2, [3000, 70], [30, 3]), (128, 8, 2, [400], [200]),  # one part, parts of the keys, many drafts
+    (64, 14, 2, [200, 1000], [30, 17]), (96, 4, 4, [300, 41], [20, 9]), (256, 8, 4, [300, 90], [12, 40]), (256, 8, 4, [3000], [12])]
+
+
+@pytest.mark.parametrize("d,hq,hkv,lens,nodes", FORMS)
+@pytest.mark.parametrize("scale", [1.0, 32.0])
+def test_a_bf16_output_is_the_rounded_fp32_one(ops, d, hq, hkv, lens, nodes, scale):
+    """No caller's choice of output or lse changes how queries and weights enter the products, whatever the size of the scores."""
+    pr = Prims(d)
+    case = build_paged_case(lens, hkv, d, 16, pr, seed=5, padded=True)
+    matrices = ancestor_matrix(nodes, random_parents(nodes, random.Random(4)))
+    mask = pack(matrices, -(-max(nodes) // 32))
+    q = (scale * torch.randn(sum(nodes), hq, d, generator=torch.Generator().manual_seed(1))).bfloat16()
+    full = _call(ops, q, case, nodes, mask, pr.cuda(), hkv, 16, out_dtype=torch.float32)
+    want, want_lse, spread = reference(q, case, nodes, matrices, pr, hkv, 16, d ** -0.5)
+    _check(full.cpu(), None, want, None, spread)
+    lse = torch.empty(sum(nodes), hq, device="cuda")
+    for kw in ({}, {"lse_out": lse}, {"mode": 3}):
+        assert torch.equal(_call(ops, q, case, nodes, mask, pr.cuda(), hkv, 16, **kw), full.bfloat16())
+
+
+@pytest.mark.parametrize("d,hq,hkv,lens,nodes", FORMS)
+def test_single_terms_where_the_caller_asks_for_them(ops, d, hq, hkv, lens, nodes):
+    pr = Prims(d)
+    p = pr.cuda()
+    case = build_paged_case(lens, hkv, d, 16, pr, seed=5, padded=True)
+    matrices = ancestor_matrix(nodes, random_parents(nodes, random.Random(4)))
+    mask = pack(matrices, -(-max(nodes) // 32))
+    q = torch.randn(sum(nodes), hq, d, generator=torch.Generator().manual_seed(1)).bfloat16()
+    want, want_lse, spread = reference(q, case, nodes, matrices, pr, hkv, 16, d ** -0.5)
+    lse = torch.empty(sum(nodes), hq, device="cuda")
+    got = _call(ops, q, case, nodes, mask, p, hkv, 16, mode=4, lse_out=lse)
+    _check(got.cpu(), lse.cpu(), want, want_lse, spread, torch.bfloat16)
+    assert torch.equal(_call(ops, q, case, nodes, mask, p, hkv, 16, mode=4), got)
+    full = _call(ops, q, case, nodes, mask, p, hkv, 16, mode=4, out_dtype=torch.float32)
+    assert torch.equal(full.bfloat16(), got)
+    # one row that sees a token without a finite norm, one query that is not finite: their rows alone
+    hurt, hurt_q = dict(case, cache=case["cache"].clone()), q.clone()
+    token = lens[0] - nodes[0] + 4
+    hurt["cache"][case["block_table"][0, token // 16].long(), token % 16][hkv * d // 2 : hkv * d // 2 + 4] = torch.tensor([math.nan]).view(torch.uint8)
+    hurt_q[9, hq - 1, 3] = math.inf
+    hit = torch.zeros(sum(nodes), hq, dtype=torch.bool)
+    hit[: nodes[0], : hq // hkv] = torch.from_numpy(matrices[0][:, 4])[:, None]
+    hit[9, hq - 1] = True
+    bad = _call(ops, hurt_q, hurt, nodes, mask, p, hkv, 16, mode=4)
+    assert torch.isnan(bad.cpu()[hit]).all() and torch.equal(bad.cpu()[~hit], got.cpu()[~hit])
+    assert ops.read_and_clear_errors(got.device) == 0
+
+
+def test_modes_that_there_are_not(ops):
+    pr, nodes = Prims(128), [6]
+    case = build_paged_case([100], 2, 128, 16, pr, seed=3, padded=True)
+    q, mask = torch.zeros(6, 8, 128, dtype=torch.float16), torch.zeros(6, 1, dtype=torch.int32)
+    for mode in (1, 2, 5, -1, 1 << 32):
+        with pytest.raises(AssertionError, match="mode"):
+            _call(ops, q, case, nodes, mask, pr.cuda(), 2, 16, mode=mode)
+    for dtype in (torch.float16, torch.float32):
+        with pytest.raises(NotImplementedError):
+            _call(ops, q.to(dtype), case, nodes, mask, pr.cuda(), 2, 16, mode=4)

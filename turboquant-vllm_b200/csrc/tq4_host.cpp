@@ -610,9 +610,9 @@ PyObject* cache_step(PyObject*, PyObject* const* p, Py_ssize_t n) {
 }
 
 // tree_attention(q, kv_cache, block_table, seq_lens, query_start_loc, tree_mask, k_centroids, v_centroids, rotation, num_kv_heads, block_size,
-//                sm_scale, sliding_window, out, out_dtype, lse_out, out_rotated, workspace, max_seq_len)
+//                sm_scale, sliding_window, out, out_dtype, lse_out, out_rotated, workspace, mode, max_seq_len)
 PyObject* tree_attention(PyObject*, PyObject* const* p, Py_ssize_t n) {
-  if (!expect("tree_attention", n, 19)) return nullptr;
+  if (!expect("tree_attention", n, 20)) return nullptr;
   return guarded([&]() -> PyObject* {
     at::Tensor q = cuda_tensor(p[0], "q");
     const int dev = device_index(q);
@@ -667,7 +667,9 @@ PyObject* tree_attention(PyObject*, PyObject* const* p, Py_ssize_t n) {
     const size_t have = (size_t)ws.numel() * ws.element_size();
     if (have < need)
       fail(PyExc_ValueError, "workspace has " + std::to_string(have) + " bytes, " + std::to_string(need) + " needed");
-    int64_t max_seq_len = p[18] == Py_None ? 0 : as_int(p[18]);
+    const int64_t mode = as_int(p[18]);
+    TQ4_ASSERT(mode == 0 || mode == 3 || mode == 4, "mode must be 0, 3 or 4");
+    int64_t max_seq_len = p[19] == Py_None ? 0 : as_int(p[19]);
     if (bt.size(1) > 0 && (max_seq_len <= 0 || max_seq_len > bt.size(1) * block)) max_seq_len = bt.size(1) * block;
     const int rotated = truth(p[16]) ? 1 : 0;
     int* flag = (int*)flag_of(dev).data_ptr();
@@ -681,7 +683,7 @@ PyObject* tree_attention(PyObject*, PyObject* const* p, Py_ssize_t n) {
           bt.stride(0), bt.size(1), (const int32_t*)lens.data_ptr(), (const int32_t*)qsl.data_ptr(), max_seq_len, (const int32_t*)mask.data_ptr(),
           mask.stride(0), (int)mask.size(1), (const float*)kc.data_ptr(), (int)kc.numel(), (const float*)vc.data_ptr(), (int)vc.numel(),
           (const float*)rot.data_ptr(), scale, window, out.data_ptr(), out_dt, out.stride(0), out.stride(1), lse, rotated, ws.data_ptr(),
-          have, flag, launch.stream);
+          have, (int)mode, flag, launch.stream);
     }
     check(st, "paged_tq4_tree_attention");
     if (!own_out) {

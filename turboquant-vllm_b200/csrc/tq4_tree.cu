@@ -113,8 +113,10 @@ extern "C" int tq4_tree_attention(
     int64_t max_seq_len, const int32_t* tree_mask, int64_t tree_mask_stride, int tree_mask_words, const float* k_centroids,
     int n_k_centroids, const float* v_centroids, int n_v_centroids, const float* rotation, float sm_scale, int sliding_window, void* out,
     int out_dtype, int64_t out_token_stride, int64_t out_head_stride, float* lse_out, int out_rotated, void* workspace,
-    size_t workspace_bytes, int* err_flag, void* stream) {
+    size_t workspace_bytes, int mode, int* err_flag, void* stream) {
   using namespace tq4;
+  if (mode != 0 && mode != 3 && mode != 4) return TQ4_ERR_INVALID_ARG;
+  if (mode == 4 && q_dtype != TQ4_BF16) return TQ4_ERR_UNSUPPORTED;
   if (num_rows < 0 || num_rows > 0x7fffffff || num_seqs < 0 || block_size <= 0 || num_blocks < 0 || bt_width < 0 || tree_mask_words < 0)
     return TQ4_ERR_INVALID_ARG;
   if (!supported_head_dim(head_dim) || q_dtype < 0 || q_dtype > 2 || out_dtype < 0 || out_dtype > 2) return TQ4_ERR_UNSUPPORTED;
@@ -178,8 +180,10 @@ extern "C" int tq4_tree_attention(
   // its CTAs on average, which would dequantise every tile again.  64 sequences of 4096 tokens, 32 / 8 heads of 128, bf16, few / other:
   // 32 drafts (128 rows) 265 / 421 us, 64 drafts 518 / 509, 128 drafts 984 / 912 (fp16: 339 / 451, 662 / 616, 1261 / 1079).
   const bool few = tree_few_supported(a) && num_rows * a.sh.G <= 128 * (int64_t)(num_seqs > 0 ? num_seqs : 1);
-  // queries and weights as single fp16 terms: half the products, where bf16 has lost more of the queries and will lose more of the output
-  const bool fast = a.q_dtype == TQ4_BF16 && out_dtype == TQ4_BF16 && !lse_out;
+  // queries, weights and Pi as single fp16 terms: the caller's choice only, as in tq4_paged_attention.  What that adds to the output's error
+  // grows with the scores and passes the rounding of a bf16 output (1.7e-3 of relative 2-norm): 5e-4, 9e-4, 1.9e-3 and 2.8e-3 at
+  // scores with a standard deviation of 1.7, 7, 28 and 55 (4096 keys, head_dim 128), where two terms have 1e-4, 1.4e-4, 2.7e-4 and 4e-4.
+  const bool fast = mode == 4;
   const int64_t slots = room / ((int64_t)num_q_heads * (head_dim + 1) * 4) - 1;
   const int splits = few ? tree_few_splits(a, slots) : tree_tc_splits(a, slots);
   const bool to_parts = splits > 1;

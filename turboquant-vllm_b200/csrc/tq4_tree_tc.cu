@@ -25,9 +25,9 @@
 // Roles: warps 0 - 3 softmax (a thread a row), 4 - 7 dequantisation, 8 the issuing thread, 9 the fetching lanes.  They meet at
 // mbarriers; every wait is bounded as in the prefill kernel.
 //
-// FAST: the terms of queries and probabilities that 11 bits leave out stay out, half the tensor work.  Used where queries and output are
-// bf16 and no lse is asked for: the queries have lost 2^-9 of a coordinate and the output will, and a rounding of 2^-12 of queries
-// and weights moves it by 4e-4 of its norm, beside 1.7e-3 of its own.  (An fp16 output's rounding is 2e-4: both terms stay.)
+// FAST: the terms of queries, probabilities and Pi that 11 bits leave out stay out, half the tensor work.  For callers that ask for it
+// (mode 4, bf16 queries): a rounding of 2^-12 of a query moves a score by that much of it, so the output's error grows with the scores,
+// from 5e-4 of its norm to more than a bf16 output's own 1.7e-3 (tq4_tree.cu has figures).
 #include <math_constants.h>
 
 #include <cstdlib>

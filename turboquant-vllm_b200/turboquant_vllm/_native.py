@@ -96,7 +96,7 @@ _SIGNATURES = {
                                    c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_int,
                                    c_void_p, c_int, c_void_p, c_int, c_void_p, c_float, c_int,
                                    c_void_p, c_int, c_int64, c_int64, c_void_p, c_int,
-                                   c_void_p, c_size_t, c_void_p, c_void_p]),
+                                   c_void_p, c_size_t, c_int, c_void_p, c_void_p]),
     "tq4_copy_blocks_workspace_bytes": (c_size_t, [c_int64, c_int64]),
     "tq4_copy_blocks": (c_int, [c_void_p, c_int, c_int64, c_int, c_int64, c_int64, c_int, c_int, c_void_p, c_int,
                                 c_int64, c_void_p, c_size_t, c_void_p, c_void_p]),

@@ -546,6 +546,7 @@ def paged_tq4_tree_attention(
     lse_out: torch.Tensor | None = None,
     out_rotated: bool = False,
     workspace: torch.Tensor | None = None,
+    mode: int = 0,
     max_seq_len: int | None = None,
 ) -> torch.Tensor:
     """Attention of trees of drafted tokens ``q [T, Hq, D]`` over the packed paged cache.
@@ -555,12 +556,13 @@ def paged_tq4_tree_attention(
     drafts those whose bits are set in its row of ``tree_mask`` (:func:`tq4_tree_mask`, or any other int32 ``[T, words]``).
     ``sliding_window``: of the keys in front of the drafts, those within the window of the row's position, which is that of the last
     of them plus the number of its set bits; the drafts are left to the mask.  A row that sees nothing gets zeros (``lse_out``: -inf).
-    The other arguments, and the precision, are those of :func:`paged_tq4_attention`; but bf16 queries with a bf16 output and no
-    ``lse_out`` may enter the tensor cores as single fp16 terms, as the weights (4e-4 of the output's norm, beside 1.7e-3 that bf16 costs).
+    The other arguments, and the precision, are those of :func:`paged_tq4_attention`.  ``mode``: 0 auto, 3 queries and probabilities as
+    two fp16 terms (what 0 takes), 4 as single ones (bf16 queries only): faster, never picked automatically, with an error that grows with
+    the scores (of the output's norm 5e-4 at scores with a standard deviation of 2, 2e-3 at 28; a bf16 output's own rounding is 1.7e-3).
     """
     return nv.host().tree_attention(
         q, kv_cache, block_table, seq_lens, query_start_loc, tree_mask, k_centroids, v_centroids, rotation, num_kv_heads, block_size,
-        sm_scale, sliding_window, out, out_dtype, lse_out, out_rotated, workspace, max_seq_len)
+        sm_scale, sliding_window, out, out_dtype, lse_out, out_rotated, workspace, mode, max_seq_len)
 
 
 # --------------------------------------------------------------------------------------
