@@ -608,3 +608,25 @@ def test_modes_that_there_are_not(ops):
     for dtype in (torch.float16, torch.float32):
         with pytest.raises(NotImplementedError):
             _call(ops, q.to(dtype), case, nodes, mask, pr.cuda(), 2, 16, mode=4)
+
+
+@pytest.mark.parametrize("d,hq,hkv,lens,nodes", [
+    (128, 4, 2, [12, 1], [20, 9]), (256, 8, 4, [12, 1], [20, 9]), (128, 8, 2, [150], [200]), (128, 28, 4, [3000], [8])])
+@pytest.mark.parametrize("window", [1 << 20, 2 ** 31 - 1, 2 ** 31, 2 ** 32 + 5])
+def test_a_window_wider_than_every_context_is_none(ops, d, hq, hkv, lens, nodes, window):
+    """Also where there are more drafts than tokens; and it leaves the choice of key parts alone."""
+    from turboquant_vllm import _native as nv
+
+    pr = Prims(d)
+    case = build_paged_case(lens, hkv, d, 16, pr, seed=3, padded=True)
+    mask = pack(ancestor_matrix(nodes, random_parents(nodes, random.Random(1), 3)), -(-max(nodes) // 32))
+    q = torch.randn(sum(nodes), hq, d, generator=torch.Generator().manual_seed(3)).half()
+    got = []
+    for w in (None, window):
+        lse = torch.empty(sum(nodes), hq, device="cuda")
+        nv.profile_start(8)
+        out = _call(ops, q, case, nodes, mask, pr.cuda(), hkv, 16, lse_out=lse, sliding_window=w)
+        got.append((out, lse, len(nv.profile_read(nv.PROF_COMBINE, 8))))
+        nv.profile_stop()
+    assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1]) and got[0][2] == got[1][2]
+    assert (got[0][1] > -math.inf).any()

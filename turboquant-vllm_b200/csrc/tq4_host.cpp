@@ -640,7 +640,8 @@ PyObject* tree_attention(PyObject*, PyObject* const* p, Py_ssize_t n) {
     if (!rot.is_contiguous()) rot = rot.contiguous();
     q = inner_contiguous(q);
     const float scale = p[11] == Py_None ? (float)(1.0 / std::sqrt((double)d)) : (float)as_double(p[11]);
-    const int window = (int)int_or_zero(p[12]);
+    const int64_t asked = int_or_zero(p[12]);  // (one past 31 bits is none, as one past the table)
+    const int window = asked > 0 && asked <= 0x7fffffff ? (int)asked : 0;
     Launch launch(dev);
     at::Tensor out;
     const bool own_out = p[13] == Py_None;

@@ -162,7 +162,8 @@ extern "C" int tq4_tree_attention(
   a.lut_scale_k = lut_scale(head_dim, n_k_centroids);
   a.lut_scale_v = lut_scale(head_dim, n_v_centroids);
   a.causal = 1;
-  a.sliding_window = sliding_window > 0 ? sliding_window : 0;
+  // (a window that every position of a row of the table lies within is none: positions minus it stay in 32 bits)
+  a.sliding_window = sliding_window > 0 && sliding_window < bt_width * block_size + 32 * (int64_t)tree_mask_words ? sliding_window : 0;
   a.out = out;
   a.out_dtype = out_dtype;
   a.out_token_stride = out_token_stride;
