@@ -198,3 +198,16 @@ def test_captured(ops):
     graph.replay()
     want = ops.tq4_rotary(q, k, pos, freq)
     assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+def test_in_place_through_another_view_of_one_token(ops):
+    """Strides of dimensions of one element say nothing: these are the same places."""
+    x = torch.randn(1, 4, 128, generator=torch.Generator().manual_seed(2)).cuda()
+    pos, freq = torch.tensor([7]).cuda(), (10000.0 ** (-torch.arange(0, 128, 2, dtype=torch.float64) / 128)).cuda()
+    want, _ = ops.tq4_rotary(x, None, pos, freq)
+    for shape, strides in (((1, 4, 128), (7, 128, 1)), ((4, 1, 128), (128, 3, 1))):
+        mine = x.clone().view(shape)
+        p = pos.expand(shape[0]).contiguous()
+        out = mine.as_strided(shape, strides)
+        assert ops.tq4_rotary(mine, None, p, freq, out=(out, None))[0] is out
+        assert torch.equal(mine.view(1, 4, 128), want)

@@ -793,7 +793,8 @@ PyObject* rotary(PyObject*, PyObject* const* p, Py_ssize_t n) {
       y[i] = on_device(cuda_tensor(out[i], "out"), dev, "out");
       TQ4_ASSERT(y[i].sizes() == x[i].sizes() && y[i].scalar_type() == x[i].scalar_type() && (d < 2 || y[i].stride(2) == 1),
                  "out must have the input's shape and type, and contiguous rows");
-      const bool same = y[i].data_ptr() == x[i].data_ptr() && y[i].strides() == x[i].strides();
+      bool same = y[i].data_ptr() == x[i].data_ptr();
+      for (int k = 0; k < 3; ++k) same = same && (y[i].size(k) < 2 || y[i].stride(k) == x[i].stride(k));
       TQ4_ASSERT(same || !overlap(y[i], x[i]), "an output must be its input or not overlap it");
       x[i] = inner_contiguous(x[i]);
     }
