@@ -57,7 +57,7 @@ typedef enum {
                                     the source of one and the destination of another; the later pair, or the one that
                                     reads it, was not carried out */
 #define TQ4_DEV_KEEP_ORDER 32 /* tq4_compact_rows: a list is not strictly increasing from 0 or more, or longer than its
-                                 row; its sequence was left as it is */
+                                 row; its sequence was left as it is, seq_lens_out is starts + keep_lens all the same */
 #define TQ4_DEV_BAD_TREE 128 /* tq4_tree_mask: a parent that is no earlier draft of its sequence (taken for none), or a
                                draft behind the mask's last bit */
 
@@ -392,7 +392,8 @@ int tq4_tree_mask(const int32_t* parents, const int32_t* query_start_loc, int64_
  * of its set bits, minus 1, and of the former it sees those within the window; the drafts are the mask's alone.
  * tree_mask int32 [num_rows, tree_mask_words] and block_table int32 [num_seqs, bt_width] with row strides in elements; a sequence
  * longer than its row of the table is cut there (TQ4_DEV_BAD_BLOCK).  max_seq_len as in tq4_attention_step; the other arguments,
- * checks and the precision are those of tq4_paged_attention in the prefill form, with at most 128 query heads per KV head.  mode: 0 or 3,
+ * checks and the precision are those of tq4_paged_attention in the prefill form, with at most 128 query heads per KV head (more, and any
+ * call with TQ4_NO_TC in the environment: TQ4_ERR_UNSUPPORTED).  mode: 0 or 3,
  * queries and probabilities enter the tensor cores as two fp16 terms; 4 (bf16 queries; never chosen by 0), as single ones, and Pi with
  * them: less tensor work, and an error that grows with the scores, 5e-4 of relative 2-norm where they have a standard deviation
  * of 2, 9e-4 at 7, 2e-3 at 28 (a bf16 output's own rounding: 1.7e-3).

@@ -20,8 +20,10 @@ struct MaskArgs {
 };
 
 // Row j of a sequence: bits of j, its parent, the parent's parent, ...  A thread walks up from one row, with the parents and the rows'
-// words in shared memory; a block then stores its rows' words side by side.  Bound by the walk, some 40 cycles a step.  (A thread for each
-// word of a row walked every branch once a word: 64 trees of 200 to 512 drafts 10.3 us, 7.2 us so.)
+// words in shared memory; a block then stores its rows' words side by side.  Bound by the walk, 0.1 us a step (the parents from shared memory,
+// behind the bit that went into it before): 64 trees of 200 to 512 drafts and chains of up to 37 7.0 us, 2.6 of them the launch and its
+// round trips, 1.1 zeroing and storing 16 words a row; 3.7 without a parent, 53 with chains of 509.  (A thread for each word of a row
+// walked every branch once a word: 10.3 us.)
 // blockIdx.x: sequence (the one behind the last stands for rows of no sequence), blockIdx.y: share of its rows
 __global__ void __launch_bounds__(kMaskThreads) tree_mask_kernel(const MaskArgs a) {
   extern __shared__ unsigned s_bits[];  // [rows of a block][pitch]
@@ -178,8 +180,10 @@ extern "C" int tq4_tree_attention(
   float* part_o = reinterpret_cast<float*>(image + prefill_tc_image_bytes(head_dim));
   const int64_t room = (int64_t)((uintptr_t)workspace + workspace_bytes) - (int64_t)(uintptr_t)part_o;
   // The kernel for few drafts takes 128 / G rows of a sequence a CTA, the other twice that: the first, unless sequences fill more than one of
-  // its CTAs on average, which would dequantise every tile again.  64 sequences of 4096 tokens, 32 / 8 heads of 128, bf16, few / other:
-  // 32 drafts (128 rows) 265 / 421 us, 64 drafts 518 / 509, 128 drafts 984 / 912 (fp16: 339 / 451, 662 / 616, 1261 / 1079).
+  // its CTAs on average, which would dequantise every tile again.  64 sequences of 4096 tokens, 32 / 8 heads of 128, few / other:
+  // 32 drafts (128 rows) 339 / 451 us, 64 drafts 662 / 616, 128 drafts 1261 / 1079 (single terms: 265 / 421, 518 / 509, 984 / 912).
+  // (Offsets are on the device: the average is over sequences with and without drafts.  One tree of many drafts among empty ones
+  // goes to the first.)
   const bool few = tree_few_supported(a) && num_rows * a.sh.G <= 128 * (int64_t)(num_seqs > 0 ? num_seqs : 1);
   // queries, weights and Pi as single fp16 terms: the caller's choice only, as in tq4_paged_attention.  What that adds to the output's error
   // grows with the scores and passes the rounding of a bf16 output (1.7e-3 of relative 2-norm): 5e-4, 9e-4, 1.9e-3 and 2.8e-3 at

@@ -12,13 +12,15 @@
 //     rotations fill the other's waits.  One K~ buffer is enough: keys are written during the softmax of the tile before.  V~ has
 //     two where there is room (all but two-term head_dim 128), which is worth 3 %;
 //   * warps without a draft take no part.
-// Measured (graph replays; in brackets the floor by bytes or operations), us: 8 drafts behind 1024 tokens of 28 / 4 heads of 128 21.1 (0.1);
-// 16 sequences of 300 to 8100 tokens, 5 to 24 drafts, 32 / 8 heads, fp16 108 (11.8); 64 of 4096 with 16 drafts, bf16 223 (46); 8 of
-// 65536 with 48 to 64 drafts, 32 / 32 heads of 96 1440 (268).  A call of few tiles is its chain: 13 thousand cycles of search, queries and
+// Measured (graph replays; in brackets single terms, mode 4; then the floor by bytes or operations), us: 8 drafts behind 1024 tokens of
+// 28 / 4 heads of 128 25 (22), 0.1; 16 sequences of 300 to 8100 tokens, 5 to 24 drafts, 32 / 8 heads, fp16 108, 11.8; 64 of 4096 with
+// 16 drafts, bf16 324 (225), 46; 8 of 65536 with 48 to 64 drafts, 32 / 32 heads of 96 1960 (1414), 268.  With two terms a CTA
+// takes some 4300 cycles a tile at head_dim 128, where there is room for one stage of rows and one V~ buffer; the tensor pipe is busy for 39 %.
+// What follows was measured with single terms.  A call of few tiles is its chain: 13 thousand cycles of search, queries and
 // rotation, 6 of the first tile, 8 of un-rotation and stores.  In long ones a CTA takes 2900 cycles a tile, for
 // keys and values (1200 and 1000) and the waits of the dequantising warps (750 with a wait for each of four barriers, 3050 in all and
 // 231 us at 64 x 4096); the softmax warps need 1600 of them, the products 530.  The load/store pipe is
-// 56 % busy with wavefronts and some 17 % more with operand reads and boxes: items of the same warps take twice as long with two
+// 60 % busy with wavefronts and some 17 % more with operand reads and boxes: items of the same warps take twice as long with two
 // CTAs as with one.  What took work off one of the groups moved it to the other, and none of it paid: rows of fewer than 64
 // twice or four times among the 128, each with its share of a tile's columns, softmax 770 cycles a tile, 247 us instead of 234 at 64 x 4096; the
 // norms by the softmax warps, 246; half of the values as well, 298; eight dequantising warps, 278; permutes for the values' table, 253.

@@ -602,6 +602,6 @@ def tq4_compact_rows(
     For ``j < keep_lens[i]`` the row at position ``starts[i] + keep[i, j]`` of sequence ``i`` goes to ``starts[i] + j``; ``keep`` int32
     ``[num_seqs, places]`` is strictly increasing in each row.  Rows behind the last one stay as they are, and so does a sequence whose
     list is out of order or longer than its row (the device's error flag says so).  The pages from ``starts[i]`` on must be sequence
-    ``i``'s alone.  ``seq_lens_out`` int32 ``[num_seqs]`` gets ``starts + keep_lens``.
+    ``i``'s alone.  ``seq_lens_out`` int32 ``[num_seqs]`` gets ``starts + keep_lens``, also for a sequence whose list was refused.
     """
     nv.host().compact_rows(kv_caches, block_table, starts, keep, keep_lens, num_kv_heads, head_dim, seq_lens_out)
