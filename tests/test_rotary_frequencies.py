@@ -158,3 +158,18 @@ def test_dynamic_scaling_of_a_single_pair_is_refused():
     with pytest.raises(ValueError, match="dynamic.*rotary_dim"):
         rotary_inv_freq(2, scaling={"rope_type": "dynamic", "factor": 2.0, "original_max_position_embeddings": 2048})
     assert rotary_inv_freq(4, scaling={"rope_type": "dynamic", "factor": 2.0, "original_max_position_embeddings": 2048})[0].shape == (2,)
+
+
+def test_modes_of_tree_attention_at_the_c_entry_point(cuda_lib):
+    """0 and 3, and 4 for bf16 queries: others are refused before anything is looked at; no rows, nothing to do."""
+    ok, invalid, unsupported = 0, 1, 2
+
+    def call(mode, q_dtype=2, rows=0):
+        return cuda_lib.tq4_tree_attention(
+            None, q_dtype, rows, 1, 8, 2, 128, 1024, 128, None, 16 * 272, 272, 8, 16, None, 4, 4, None, None, 0, None, 1, 1, None, 16, None, 16, None,
+            0.1, 0, None, 2, 1024, 128, None, 0, None, 0, mode, None, None)
+
+    assert [call(mode) for mode in (0, 3, 4)] == [ok] * 3
+    assert [call(mode) for mode in (1, 2, 5, -1)] == [invalid] * 4
+    assert call(4, q_dtype=1) == call(4, q_dtype=0) == unsupported
+    assert call(0, rows=3) == call(4, rows=3) == invalid
