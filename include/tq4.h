@@ -394,9 +394,9 @@ int tq4_tree_mask(const int32_t* parents, const int32_t* query_start_loc, int64_
  * longer than its row of the table is cut there (TQ4_DEV_BAD_BLOCK).  max_seq_len as in tq4_attention_step; the other arguments,
  * checks and the precision are those of tq4_paged_attention in the prefill form, with at most 128 query heads per KV head (more, and any
  * call with TQ4_NO_TC in the environment: TQ4_ERR_UNSUPPORTED).  mode: 0 or 3,
- * queries and probabilities enter the tensor cores as two fp16 terms; 4 (bf16 queries; never chosen by 0), as single ones, and Pi with
- * them: less tensor work, and an error that grows with the scores, 5e-4 of relative 2-norm where they have a standard deviation
- * of 2, 9e-4 at 7, 2e-3 at 28 (a bf16 output's own rounding: 1.7e-3).
+ * queries and probabilities enter the tensor cores as two fp16 terms; 4 (bf16 queries; never chosen by 0), as single ones, for few
+ * drafts Pi with them: less tensor work, and an error that grows with the scores, 5e-4 of relative 2-norm where they have a standard
+ * deviation of 2, 9e-4 at 7, 2e-3 at 28 (a bf16 output's own rounding: 1.7e-3).
  * A row that sees no key, or past the last offset, gets zeros and an lse of -inf.  An infinite or NaN norm in the cache makes the rows
  * that see its token NaN, output and lse, and no others.
  * workspace >= tq4_tree_attention_workspace_bytes(num_rows, Hq, Hkv, D), 16-byte aligned.

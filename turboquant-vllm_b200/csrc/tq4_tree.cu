@@ -185,7 +185,7 @@ extern "C" int tq4_tree_attention(
   // (Offsets are on the device: the average is over sequences with and without drafts.  One tree of many drafts among empty ones
   // goes to the first.)
   const bool few = tree_few_supported(a) && num_rows * a.sh.G <= 128 * (int64_t)(num_seqs > 0 ? num_seqs : 1);
-  // queries, weights and Pi as single fp16 terms: the caller's choice only, as in tq4_paged_attention.  What that adds to the output's error
+  // queries, weights and (few drafts) Pi as single fp16 terms: the caller's choice only, as in tq4_paged_attention.  What that adds to the output's error
   // grows with the scores and passes the rounding of a bf16 output (1.7e-3 of relative 2-norm): 5e-4, 9e-4, 1.9e-3 and 2.8e-3 at
   // scores with a standard deviation of 1.7, 7, 28 and 55 (4096 keys, head_dim 128), where two terms have 1e-4, 1.4e-4, 2.7e-4 and 4e-4.
   const bool fast = mode == 4;
